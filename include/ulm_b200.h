@@ -25,6 +25,9 @@
  *   run.c:121-265      run.c reset_state / forward            -> ulm_decode_* (batched)
  *   run.c:460-534      run.c sample (argmax / mult / top-p)   -> ulm_decode_head, ulm_decode_sample
  *   model.py:153-157   output Linear + F.cross_entropy        -> ulm_lm_head_loss_fwd, _bwd
+ *   model.py:153-157   output Linear (+ log_softmax, gather)   -> ulm_lm_head_logprobs_*, ulm_token_logprobs_*
+ *   model.py:149-150   tok_embeddings and its gradient         -> ulm_embedding_fwd, _bwd
+ *   train.py:284       clip_grad_norm_ of the training loop    -> ulm_clip_grads
  */
 #ifndef ULM_B200_H
 #define ULM_B200_H
@@ -437,6 +440,64 @@ int64_t ulm_decode_prefill_work_bytes(int64_t B, int64_t T, int64_t D, int prec)
 int ulm_decode_sample(const float* logits, int64_t B, int64_t V, float temperature, float topp,
                       unsigned long long* rng_state, int* next_token, const void* emb, int emb_dtype, float* x,
                       int64_t D, void* stream);
+
+/* ---- log probabilities of given tokens (model.py:153-157's logits, log_softmax and gather) -------- */
+
+/* Per row r of logits x (N,V) of dtype with row stride ld, with m = max_v x_v and
+ * s = sum_v exp(x_v - m): logprobs[r] = (x_t - m) - log s for the row's token t = tokens[r],
+ * entropy[r] = the entropy of softmax(x), and the top_k best tokens (value descending, lower id
+ * first among equals, NaN above all) in top_ids and top_logprobs (N,top_k), 0 <= top_k <= min(V, 32).
+ * Token -1 is padding: its logprob is 0 (entropy and top_k are the row's own). Any other token
+ * outside [0,V) gives a NaN logprob. Logits of -inf are masked tokens; a row with nothing else, or
+ * with a NaN or +inf, has NaN results, as log_softmax has (its top_ids still follow the order above).
+ * stats (N,2) fp32: (m, log s), what the backward needs; may be NULL. */
+int ulm_token_logprobs_fwd(const void* logits, int dtype, int64_t ld, const int64_t* tokens, float* logprobs,
+                           float* entropy, float* stats, int64_t* top_ids, float* top_logprobs, int64_t N, int64_t V,
+                           int top_k, void* stream);
+/* Backward: dlogits (N,V) of dtype, row stride ld_d, from the gradients of logprobs and entropy (either
+ * may be NULL: none). stats and entropy as the forward left them. */
+int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* logits, int dtype, int64_t ld,
+                           const int64_t* tokens, const float* stats, const float* entropy, void* dlogits, int64_t ld_d,
+                           int64_t N, int64_t V, void* stream);
+
+/* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd.
+ * work: ulm_lm_head_logprobs_work_bytes(N,V,D,0,prec) bytes. */
+int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens,
+                             float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
+                             void* work, int64_t N, int64_t V, int64_t D, int top_k, int prec, void* stream);
+/* Backward: dh (N,D) of dh_dtype and dw (V,D) of dw_dtype (either may be NULL: not wanted); the logits
+ * are recomputed. work:
+ * ulm_lm_head_logprobs_work_bytes(N,V,D,1,prec) bytes. */
+int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
+                             const void* w_op, int64_t ld_w, const int64_t* tokens, const float* stats,
+                             const float* entropy, void* dh, int dh_dtype, void* dw, int dw_dtype, void* work,
+                             int64_t N, int64_t V, int64_t D, int prec, void* stream);
+int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int backward, int prec);
+
+/* ---- token embedding (nn.Embedding, model.py:119, 149) ------------------------------------------- */
+
+/* y[n] = scale * weight[tokens[n]] (N,D) of y_dtype; weight (V,D) of w_dtype, row stride ld_w. Token -1
+ * is padding and gives a zero row; any other token outside [0,V) gives a NaN row. */
+int ulm_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, int64_t ld_w, void* y, int y_dtype,
+                      int64_t N, int64_t V, int64_t D, float scale, void* stream);
+/* Backward: dw (V,D) of dw_dtype (overwritten) = scale * the sum of dy's rows (N,D) of dy_dtype by
+ * token, in fp32 and in a fixed order; tokens outside [0,V) add nothing. work:
+ * ulm_embedding_bwd_work_bytes(N,V,D) bytes. */
+int ulm_embedding_bwd(const int64_t* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, void* work,
+                      int64_t N, int64_t V, int64_t D, float scale, void* stream);
+int64_t ulm_embedding_bwd_work_bytes(int64_t N, int64_t V, int64_t D);
+
+/* ---- global gradient norm and clipping (clip_grad_norm_, train.py:284) ------------------- */
+
+/* norm (1,) fp32 = the 2-norm over all n tensors of grads (device pointers, element counts and element
+ * types in host arrays; each tensor contiguous). With outs: outs[i] = grads[i] * min(1, max_norm /
+ * (norm + 1e-6)) in out_dtypes[i]; outs[i] may be grads[i] itself (in place, the same type), else the
+ * outputs overlap neither each other nor any gradient. outs and out_dtypes NULL: the norm alone
+ * (max_norm unused). Squares are added in fp64 in a fixed order. max_norm >= 0. work:
+ * ulm_clip_grads_work_bytes(n) bytes, 8-byte aligned. */
+int ulm_clip_grads(const void* const* grads, void* const* outs, const int64_t* counts, const int* in_dtypes,
+                   const int* out_dtypes, int64_t n, float max_norm, float* norm, void* work, void* stream);
+int64_t ulm_clip_grads_work_bytes(int64_t n);
 
 #ifdef __cplusplus
 }

@@ -76,6 +76,17 @@ SIGNATURES = {
     "ulm_decode_head_work_bytes": (_I64, [_I64, _I64]),
     "ulm_decode_prefill_block": (_I, [_P] * 7 + [_I] + [_P] * 7 + [_I64] * 5 + [_I, _P]),
     "ulm_decode_prefill_work_bytes": (_I64, [_I64, _I64, _I64, _I]),
+    "ulm_token_logprobs_fwd": (_I, [_P, _I, _I64] + [_P] * 6 + [_I64, _I64, _I, _P]),
+    "ulm_token_logprobs_bwd": (_I, [_P, _P, _P, _I, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "ulm_lm_head_logprobs_fwd": (_I, [_P, _I64, _P, _I64] + [_P] * 7 + [_I64, _I64, _I64, _I, _I, _P]),
+    "ulm_lm_head_logprobs_bwd": (_I, [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I, _P,
+                                      _I64, _I64, _I64, _I, _P]),
+    "ulm_lm_head_logprobs_work_bytes": (_I64, [_I64, _I64, _I64, _I, _I]),
+    "ulm_embedding_fwd": (_I, [_P, _P, _I, _I64, _P, _I, _I64, _I64, _I64, ctypes.c_float, _P]),
+    "ulm_embedding_bwd": (_I, [_P, _P, _I, _P, _I, _P, _I64, _I64, _I64, ctypes.c_float, _P]),
+    "ulm_embedding_bwd_work_bytes": (_I64, [_I64, _I64, _I64]),
+    "ulm_clip_grads": (_I, [_P, _P, _P, _P, _P, _I64, ctypes.c_float, _P, _P, _P]),
+    "ulm_clip_grads_work_bytes": (_I64, [_I64]),
 }
 
 _lib = None

@@ -1,0 +1,88 @@
+"""The global gradient norm over many tensors, and clipping by it, on sm_100a (train.py:284).
+
+    norm = sqrt(sum over all gradients of g^2),   g <- g * min(1, max_norm / (norm + 1e-6))
+
+as torch.nn.utils.clip_grad_norm_ with the 2-norm, without a host synchronisation: `clip_grad_norm_`
+takes parameters, `clip_grads` a list of gradients (in place, or into other tensors and types, such
+as `GradBucket`'s views), `grad_norm` only measures. Squares are added in fp64 in a fixed order, so
+the norm is the same in every run. A norm that is not finite makes the factor what IEEE division
+gives (0 or NaN), as torch's function does. The work runs in libulm_b200.so (ulm_clip_grads) on the
+current stream. No CPU path.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib as L
+
+
+def _run(grads, outs, max_norm):
+    dev = grads[0].device
+    n = len(grads)
+    for g in grads:
+        if not g.is_cuda:
+            raise RuntimeError("gradient clipping runs on CUDA tensors only (no CPU path)")
+        if g.device != dev:
+            raise ValueError(f"gradients on {dev} and {g.device}: one device expected")
+        if g.layout != torch.strided:
+            raise ValueError("sparse gradients are not supported")
+    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dst = None
+    if outs is not None:
+        dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
+               for g, s, o in zip(grads, src, outs)]
+    vp, i64, i32 = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    work = torch.empty(int(L.lib().ulm_clip_grads_work_bytes(n)), device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        L.check(L.lib().ulm_clip_grads(
+            vp(*[t.data_ptr() for t in src]), vp(*[t.data_ptr() for t in dst]) if dst else None,
+            i64(*[t.numel() for t in src]), i32(*[L.dtype_code(t.dtype) for t in src]),
+            i32(*[L.dtype_code(t.dtype) for t in dst]) if dst else None, n, max_norm, L.ptr(norm), L.ptr(work),
+            L.stream_of(norm)))
+    if dst:
+        for o, d in zip(outs, dst):
+            if d is not o:
+                o.copy_(d)
+        torch.autograd.graph.increment_version(outs)
+    return norm
+
+
+def grad_norm(grads):
+    """The 2-norm over all tensors of `grads` (fp32 or bf16, one GPU), a 0-d fp32 tensor."""
+    grads = [g.detach() for g in grads if g is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    return _run(grads, None, 0.0)
+
+
+def clip_grads(grads, max_norm, out=None):
+    """Scales `grads` (fp32 or bf16 tensors of one GPU) to a 2-norm of at most `max_norm`, in place, or
+    into the tensors `out` of the same shapes (fp32 or bf16 each). Returns the norm that they had, a 0-d
+    fp32 tensor. A tensor may stand in the list once: one that is there twice, or overlaps another, is
+    refused."""
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
+    for g, o in zip(grads, outs):
+        if o.shape != g.shape:
+            raise ValueError(f"output {tuple(o.shape)} for a gradient {tuple(g.shape)}")
+        if o.device != g.device:
+            raise ValueError(f"output on {o.device} for a gradient on {g.device}")
+    if not grads:
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        return _run(grads, outs, max_norm)
+
+
+def clip_grad_norm_(parameters, max_norm):
+    """Clips the gradients of `parameters` (a tensor or an iterable of them; those without a gradient are
+    passed over) in place. Returns the norm that they had."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm)

@@ -1,0 +1,485 @@
+// Log probabilities of given tokens, with the distribution's entropy and its best alternatives:
+//   m = max_v x_v, s = sum_v exp(x_v - m), u = sum_v exp(x_v - m) (x_v - m)
+//   logp_t = (x_t - m) - log s,   H = log s - u / s,   top k by (value descending, id ascending)
+// and backward, from the gradients a of logp_t and b of H:
+//   dx_v = a ([v = t] - p_v) - b p_v (log p_v + H),   p_v = exp((x_v - m) - log s)
+// over rows of logits x that exist already (ulm_token_logprobs_*), or that are x = h W^T
+// (ulm_lm_head_logprobs_*). Token -1 is padding: logp 0 and no a term. Any other token outside
+// [0, V) makes its row's logp and gradients NaN. All statistics are fp32.
+#include "gemm.cuh"
+
+namespace ulm {
+namespace {
+
+constexpr int LP_THREADS = 256;
+constexpr int LP_GROUPS = 64;     // groups of threads whose maxima give the threshold of the top k
+constexpr int LP_CAP = 512;       // candidates of one row above the threshold
+constexpr int LP_MAX_TOP = 32;    // top_k of the entries
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Running statistics of a set of logits: the maximum m (-inf for none), s = sum exp(x - m) and
+// u = sum exp(x - m) (x - m), taken about 0 while m is -inf (every term is then zero, or NaN).
+struct LpStat {
+  float m, s, u;
+};
+
+__device__ __forceinline__ LpStat lp_merge(const LpStat& a, const LpStat& b) {
+  const float M = fmaxf(a.m, b.m);
+  auto part = [M](const LpStat& p, float& s, float& u) {
+    const float d = p.m == -INFINITY ? 0.f : p.m - M;
+    const float f = fast_exp2(d * LOG2E);
+    s = p.s * f;
+    u = f > 0.f ? (p.u + p.s * d) * f : 0.f;
+  };
+  float sa, ua, sb, ub;
+  part(a, sa, ua);
+  part(b, sb, ub);
+  return LpStat{M, sa + sb, ua + ub};
+}
+
+// NV more logits into a thread's statistics. fmaxf on the factor of u keeps exp(-inf) * -inf at 0.
+template <int NV>
+__device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
+  float lm = x[0];
+#pragma unroll
+  for (int i = 1; i < NV; ++i) lm = fmaxf(lm, x[i]);
+  if (lm > st.m) {
+    const float d = st.m == -INFINITY ? 0.f : st.m - lm;
+    const float f = fast_exp2(d * LOG2E);
+    st.u = f > 0.f ? (st.u + st.s * d) * f : 0.f;
+    st.s *= f;
+    st.m = lm;
+  }
+  const float base = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const float d = x[i] - base;
+    const float e = fast_exp2(d * LOG2E);
+    st.s += e;
+    st.u = fmaf(e, fmaxf(d, -1e4f), st.u);
+  }
+}
+
+// Order of the alternatives as one integer: the value's bits made monotone (NaN above all, -0 = 0),
+// then the lower id.
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t id) {
+  uint32_t b = __float_as_uint(x + 0.f);
+  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  if (x != x) b = 0xFFFFFFFEu;
+  return ((uint64_t)b << 32) | (uint64_t)(0xFFFFFFFFu - id);
+}
+__device__ __forceinline__ float lp_key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  if (b == 0xFFFFFFFEu) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float((b & 0x80000000u) ? (b & 0x7FFFFFFFu) : ~b);
+}
+__device__ __forceinline__ uint32_t lp_key_id(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
+
+template <typename T>
+__device__ __forceinline__ float lp_load(const T* p);
+template <>
+__device__ __forceinline__ float lp_load<float>(const float* p) {
+  return *p;
+}
+template <>
+__device__ __forceinline__ float lp_load<__nv_bfloat16>(const __nv_bfloat16* p) {
+  return __bfloat162float(*p);
+}
+
+// Logits of 16 bytes as floats.
+template <typename T>
+struct LpVec;
+template <>
+struct LpVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[4]) {
+    x[0] = __uint_as_float(q.x);
+    x[1] = __uint_as_float(q.y);
+    x[2] = __uint_as_float(q.z);
+    x[3] = __uint_as_float(q.w);
+  }
+};
+template <>
+struct LpVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+};
+
+// Elements before the first 16-byte boundary of a row, at most n.
+template <typename T>
+__device__ __forceinline__ int lp_head(const T* row, int n) {
+  const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T));
+  return h < n ? h : n;
+}
+
+// f(id, values) over the row's V logits, 16 bytes at a time from its first 16-byte boundary, and one
+// at a time at the two ends; thread t takes every LP_THREADS-th piece.
+template <typename T, typename F1, typename FV>
+__device__ __forceinline__ void lp_for_each(const T* row, int V, F1&& one, FV&& vec) {
+  constexpr int NV = LpVec<T>::N;
+  const int head = lp_head(row, V), nvec = (V - head) / NV, tail0 = head + nvec * NV;
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  if ((int)threadIdx.x < head) one((int)threadIdx.x, lp_load(row + threadIdx.x));
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nvec; i += LP_THREADS) {
+    float x[NV];
+    LpVec<T>::unpack(body[i], x);
+    vec(head + i * NV, x);
+  }
+  if (tail0 + (int)threadIdx.x < V) one(tail0 + (int)threadIdx.x, lp_load(row + tail0 + threadIdx.x));
+}
+
+// The row's logp of its token from its statistics.
+template <typename T>
+__device__ __forceinline__ float lp_given(const T* row, int64_t t, int V, float base, float logs) {
+  if (t == -1) return 0.f;
+  if (t < 0 || t >= V) return __uint_as_float(0x7FC00000u);
+  return (lp_load(row + t) - base) - logs;
+}
+
+// One CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS)
+    lp_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens,
+                   float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ stats,
+                   int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int V, int k) {
+  __shared__ LpStat part[LP_THREADS / 32];
+  __shared__ float gmax[LP_GROUPS];
+  __shared__ float thr_s;
+  __shared__ uint64_t cand[LP_CAP];
+  __shared__ uint64_t red[LP_THREADS / 32];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
+  const int64_t r = blockIdx.x;
+  const T* row = x + r * ld;
+  LpStat st{-INFINITY, 0.f, 0.f};
+  lp_for_each(
+      row, V,
+      [&](int, float v) {
+        const float one[1] = {v};
+        lp_add(st, one);
+      },
+      [&](int, const auto& v) { lp_add(st, v); });
+  // the maxima of the groups of LP_THREADS / LP_GROUPS neighbouring threads
+  float g = st.m;
+#pragma unroll
+  for (int o = LP_THREADS / LP_GROUPS / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  if (tid % (LP_THREADS / LP_GROUPS) == 0) gmax[tid / (LP_THREADS / LP_GROUPS)] = g;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const LpStat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                       __shfl_xor_sync(0xffffffffu, st.u, o)};
+    st = lp_merge(st, other);
+  }
+  if (lane == 0) part[wp] = st;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  LpStat all = part[0];
+#pragma unroll
+  for (int w = 1; w < LP_THREADS / 32; ++w) all = lp_merge(all, part[w]);
+  const float base = all.m == -INFINITY ? 0.f : all.m;
+  const float logs = logf(all.s);
+  if (tid == 0) {
+    logprobs[r] = lp_given(row, tokens[r], V, base, logs);
+    entropy[r] = logs - all.u / all.s;
+    if (stats) {
+      stats[2 * r] = base;
+      stats[2 * r + 1] = logs;
+    }
+  }
+  if (k == 0) return;
+  // The k-th largest group maximum bounds the k-th best logit from below: only logits not under it
+  // are candidates (about k of them, unless many are equal).
+  if (tid < LP_GROUPS) {
+    int rank = 0;
+    const float mine = gmax[tid];
+#pragma unroll 8
+    for (int j = 0; j < LP_GROUPS; ++j) rank += (gmax[j] > mine || (gmax[j] == mine && j < tid)) ? 1 : 0;
+    if (rank == k - 1) thr_s = mine;
+  }
+  __syncthreads();
+  const float thr = thr_s;
+  auto offer = [&](int id, float v) {
+    if (!(v < thr)) {
+      const int at = atomicAdd(&count, 1);
+      if (at < LP_CAP) cand[at] = lp_key(v, (uint32_t)id);
+    }
+  };
+  lp_for_each(row, V, offer, [&](int id, const auto& v) {
+#pragma unroll
+    for (int i = 0; i < LpVec<T>::N; ++i) offer(id + i, v[i]);
+  });
+  __syncthreads();
+  const int n = count;
+  if (n <= LP_CAP) {
+    // each candidate's place is the number of better ones
+    for (int c = tid; c < n; c += LP_THREADS) {
+      const uint64_t key = cand[c];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
+      if (rank < k) {
+        top_ids[r * k + rank] = lp_key_id(key);
+        top_logprobs[r * k + rank] = (lp_key_value(key) - base) - logs;
+      }
+    }
+    return;
+  }
+  // many equal logits: the best one after the last, k times
+  uint64_t last = ~0ull;
+  for (int j = 0; j < k; ++j) {
+    uint64_t best = 0;
+    auto look = [&](int id, float v) {
+      const uint64_t key = lp_key(v, (uint32_t)id);
+      if (key < last && key > best) best = key;
+    };
+    lp_for_each(row, V, look, [&](int id, const auto& v) {
+#pragma unroll
+      for (int i = 0; i < LpVec<T>::N; ++i) look(id + i, v[i]);
+    });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+      best = other > best ? other : best;
+    }
+    __syncthreads();
+    if (lane == 0) red[wp] = best;
+    __syncthreads();
+    best = red[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 32; ++w) best = red[w] > best ? red[w] : best;
+    last = best;
+    if (tid == 0) {
+      top_ids[r * k + j] = lp_key_id(best);
+      top_logprobs[r * k + j] = (lp_key_value(best) - base) - logs;
+    }
+  }
+}
+
+// The backward's factors of one row: dx_v = ([v = t] a) - p_v (a + b (log p_v + H)).
+struct LpCoef {
+  float base, logs, c0, b, a;
+  int64_t t;
+};
+__device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* stats, const float* entropy,
+                                          const float* dlogprobs, const float* dentropy, int64_t r, int V) {
+  LpCoef c;
+  c.t = tokens[r];
+  c.base = stats[2 * r];
+  c.logs = stats[2 * r + 1];
+  c.a = c.t == -1 || !dlogprobs ? 0.f : dlogprobs[r];
+  if (c.t < -1 || c.t >= V) c.a = __uint_as_float(0x7FC00000u);
+  c.b = dentropy ? dentropy[r] : 0.f;
+  c.c0 = c.a + (c.b != 0.f ? c.b * entropy[r] : 0.f);
+  return c;
+}
+__device__ __forceinline__ float lp_dlogit(const LpCoef& c, float x, int64_t v) {
+  const float logp = (x - c.base) - c.logs;
+  const float p = fast_exp2(logp * LOG2E);
+  const float d = p == 0.f ? 0.f : p * (c.b != 0.f ? fmaf(c.b, logp, c.c0) : c.c0);
+  return (v == c.t ? c.a : 0.f) - d;
+}
+
+template <typename T>
+__device__ __forceinline__ void lp_store(T* p, float v);
+template <>
+__device__ __forceinline__ void lp_store<float>(float* p, float v) {
+  *p = v;
+}
+template <>
+__device__ __forceinline__ void lp_store<__nv_bfloat16>(__nv_bfloat16* p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
+
+template <typename T, typename TO>
+__global__ void __launch_bounds__(LP_THREADS)
+    lp_rows_bwd_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens,
+                       const float* __restrict__ stats, const float* __restrict__ entropy,
+                       const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
+                       TO* __restrict__ dx, int64_t ld_dx, int V) {
+  const int64_t r = blockIdx.x;
+  const LpCoef c = lp_coef(tokens, stats, entropy, dlogprobs, dentropy, r, V);
+  for (int v = threadIdx.x; v < V; v += LP_THREADS)
+    lp_store(dx + r * ld_dx + v, lp_dlogit(c, lp_load(x + r * ld + v), v));
+}
+
+int lp_rows_fwd(const void* x, int dtype, int64_t ld, const int64_t* tokens, float* logprobs, float* entropy,
+                float* stats, int64_t* top_ids, float* top_logprobs, int64_t N, int64_t V, int k, cudaStream_t st) {
+  if (dtype == ULM_F32)
+    lp_rows_kernel<float><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const float*>(x), ld, tokens, logprobs, entropy,
+                                                              stats, top_ids, top_logprobs, (int)V, k);
+  else
+    lp_rows_kernel<__nv_bfloat16><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ld, tokens,
+                                                                      logprobs, entropy, stats, top_ids, top_logprobs,
+                                                                      (int)V, k);
+  ULM_LAUNCH_CHECK("lp_rows_kernel");
+  return ULM_OK;
+}
+
+template <typename T, typename TO>
+int lp_rows_bwd_t(const void* x, int64_t ld, const int64_t* tokens, const float* stats, const float* entropy,
+                  const float* dlogprobs, const float* dentropy, void* dx, int64_t ld_dx, int64_t N, int64_t V,
+                  cudaStream_t st) {
+  lp_rows_bwd_kernel<T, TO><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const T*>(x), ld, tokens, stats, entropy,
+                                                                dlogprobs, dentropy, static_cast<TO*>(dx), ld_dx,
+                                                                (int)V);
+  ULM_LAUNCH_CHECK("lp_rows_bwd_kernel");
+  return ULM_OK;
+}
+
+int lp_check(const int64_t* tokens, int64_t N, int64_t V) {
+  ULM_REQUIRE(N >= 0 && V > 0, "bad extents N=%lld V=%lld", (long long)N, (long long)V);
+  ULM_REQUIRE(N < (1ll << 31) && V < (1 << 30), "extent too large");
+  ULM_REQUIRE(N == 0 || tokens, "null tokens");
+  return ULM_OK;
+}
+
+int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const float* top_logprobs) {
+  ULM_REQUIRE(k >= 0 && k <= LP_MAX_TOP && k <= V, "top_k=%d must be in 0 .. min(V, %d)", k, LP_MAX_TOP);
+  ULM_REQUIRE(N == 0 || k == 0 || (top_ids && top_logprobs), "top_k > 0 needs top_ids and top_logprobs");
+  return ULM_OK;
+}
+
+bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
+
+inline int64_t lp_al(int64_t n) { return (n + 255) / 256 * 256; }
+inline int64_t lp_ld_logits(int64_t V) { return (V + 3) / 4 * 4; }
+// rows of logits held at once by the head entries
+int64_t lp_rows_at_once(int64_t N, int64_t V) {
+  int64_t r = (256ll << 20) / (lp_ld_logits(V) * 4) / 256 * 256;
+  r = r < 256 ? 256 : r;
+  return r < N ? r : N;
+}
+
+int lp_head_check(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens, int64_t N,
+                  int64_t V, int64_t D, int prec) {
+  ULM_REQUIRE(prec == ULM_PREC_BF16 || prec == ULM_PREC_FP32, "prec must be ULM_PREC_BF16 or ULM_PREC_FP32");
+  if (int rc = lp_check(tokens, N, V)) return rc;
+  ULM_REQUIRE(D > 0 && D < (1 << 30), "bad extent D=%lld", (long long)D);
+  ULM_REQUIRE(N == 0 || (h_op && w_op), "null pointer argument");
+  ULM_REQUIRE(ld_h >= D && ld_w >= D, "row stride shorter than the row");
+  return ULM_OK;
+}
+
+// logits of rows r0 .. r0 + n
+int lp_logits(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, int dt, float* logits, int64_t r0,
+              int64_t n, int64_t V, int64_t D, cudaStream_t st) {
+  const int64_t es = dt == ULM_F32 ? 4 : 2, ldl = lp_ld_logits(V);
+  Operand A{static_cast<const char*>(h_op) + r0 * ld_h * es, ld_h, n * ld_h, D, n, dt, false};
+  Operand Bw{w_op, ld_w, V * ld_w, D, V, dt, false};
+  GemmShape s{1, (int)n, (int)V, (int)D, CAUSAL_NONE};
+  return run_gemm(A, Bw, s, make_epilogue(EPI_STORE, ULM_F32, logits, ldl, n * ldl, nullptr), st);
+}
+
+}  // namespace
+}  // namespace ulm
+
+using namespace ulm;
+
+extern "C" int ulm_token_logprobs_fwd(const void* logits, int dtype, int64_t ld, const int64_t* tokens,
+                                      float* logprobs, float* entropy, float* stats, int64_t* top_ids,
+                                      float* top_logprobs, int64_t N, int64_t V, int top_k, void* stream) {
+  if (int rc = lp_check(tokens, N, V)) return rc;
+  if (int rc = lp_check_top(N, V, top_k, top_ids, top_logprobs)) return rc;
+  ULM_REQUIRE(lp_dtype_ok(dtype), "bad dtype");
+  ULM_REQUIRE(ld >= V, "row stride shorter than the row");
+  if (N == 0) return ULM_OK;
+  ULM_REQUIRE(logits && logprobs && entropy, "null pointer argument");
+  return lp_rows_fwd(logits, dtype, ld, tokens, logprobs, entropy, stats, top_ids, top_logprobs, N, V, top_k,
+                     static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* logits, int dtype,
+                                      int64_t ld, const int64_t* tokens, const float* stats, const float* entropy,
+                                      void* dlogits, int64_t ld_d, int64_t N, int64_t V, void* stream) {
+  if (int rc = lp_check(tokens, N, V)) return rc;
+  ULM_REQUIRE(lp_dtype_ok(dtype), "bad dtype");
+  ULM_REQUIRE(ld >= V && ld_d >= V, "row stride shorter than the row");
+  if (N == 0) return ULM_OK;
+  ULM_REQUIRE(logits && stats && entropy && dlogits, "null pointer argument");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == ULM_F32 ? lp_rows_bwd_t<float, float>(logits, ld, tokens, stats, entropy, dlogprobs, dentropy,
+                                                        dlogits, ld_d, N, V, st)
+                          : lp_rows_bwd_t<__nv_bfloat16, __nv_bfloat16>(logits, ld, tokens, stats, entropy, dlogprobs,
+                                                                        dentropy, dlogits, ld_d, N, V, st);
+}
+
+extern "C" int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int backward, int prec) {
+  if (N < 0 || V < 0 || D < 0) return -1;
+  const int64_t logits = lp_al(lp_rows_at_once(N, V) * lp_ld_logits(V) * 4);
+  return logits + (backward ? lp_al(N * ulm_operand_ld(V) * (prec == ULM_PREC_FP32 ? 4 : 2)) : 0);
+}
+
+extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w,
+                                        const int64_t* tokens, float* logprobs, float* entropy, float* stats,
+                                        int64_t* top_ids, float* top_logprobs, void* work, int64_t N, int64_t V,
+                                        int64_t D, int top_k, int prec, void* stream) {
+  if (int rc = lp_head_check(h_op, ld_h, w_op, ld_w, tokens, N, V, D, prec)) return rc;
+  if (int rc = lp_check_top(N, V, top_k, top_ids, top_logprobs)) return rc;
+  if (N == 0) return ULM_OK;
+  ULM_REQUIRE(logprobs && entropy && work, "null pointer argument");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int dt = prec == ULM_PREC_FP32 ? ULM_F32 : ULM_BF16;
+  float* logits = static_cast<float*>(work);
+  const int64_t step = lp_rows_at_once(N, V);
+  for (int64_t r0 = 0; r0 < N; r0 += step) {
+    const int64_t n = N - r0 < step ? N - r0 : step;
+    if (int rc = lp_logits(h_op, ld_h, w_op, ld_w, dt, logits, r0, n, V, D, st)) return rc;
+    if (int rc = lp_rows_fwd(logits, ULM_F32, lp_ld_logits(V), tokens + r0, logprobs + r0, entropy + r0,
+                             stats ? stats + 2 * r0 : nullptr, top_ids ? top_ids + r0 * top_k : nullptr,
+                             top_logprobs ? top_logprobs + r0 * top_k : nullptr, n, V, top_k, st))
+      return rc;
+  }
+  return ULM_OK;
+}
+
+extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
+                                        const void* w_op, int64_t ld_w, const int64_t* tokens, const float* stats,
+                                        const float* entropy, void* dh, int dh_dtype, void* dw, int dw_dtype,
+                                        void* work, int64_t N, int64_t V, int64_t D, int prec, void* stream) {
+  if (int rc = lp_head_check(h_op, ld_h, w_op, ld_w, tokens, N, V, D, prec)) return rc;
+  ULM_REQUIRE(lp_dtype_ok(dh_dtype) && lp_dtype_ok(dw_dtype), "bad dtype");
+  ULM_REQUIRE(N == 0 || (stats && entropy && work), "null pointer argument");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!dh && !dw) return ULM_OK;
+  if (N == 0) {
+    if (dw) ULM_CUDA_TRY(cudaMemsetAsync(dw, 0, V * D * (dw_dtype == ULM_F32 ? 4 : 2), st));
+    return ULM_OK;
+  }
+  const int dt = prec == ULM_PREC_FP32 ? ULM_F32 : ULM_BF16;
+  const int64_t es = dt == ULM_F32 ? 4 : 2, ldv = ulm_operand_ld(V), step = lp_rows_at_once(N, V);
+  float* logits = static_cast<float*>(work);
+  char* dlogits = static_cast<char*>(work) + lp_al(step * lp_ld_logits(V) * 4);
+  for (int64_t r0 = 0; r0 < N; r0 += step) {
+    const int64_t n = N - r0 < step ? N - r0 : step;
+    if (int rc = lp_logits(h_op, ld_h, w_op, ld_w, dt, logits, r0, n, V, D, st)) return rc;
+    void* d = dlogits + r0 * ldv * es;
+    const float* da = dlogprobs ? dlogprobs + r0 : nullptr;
+    const float* db = dentropy ? dentropy + r0 : nullptr;
+    const int rc = dt == ULM_F32
+                       ? lp_rows_bwd_t<float, float>(logits, lp_ld_logits(V), tokens + r0, stats + 2 * r0, entropy + r0,
+                                                     da, db, d, ldv, n, V, st)
+                       : lp_rows_bwd_t<float, __nv_bfloat16>(logits, lp_ld_logits(V), tokens + r0, stats + 2 * r0,
+                                                             entropy + r0, da, db, d, ldv, n, V, st);
+    if (rc) return rc;
+  }
+  if (dh) {
+    // dh = dx W: A = dx (rows, K-major over the vocabulary), B = W as [token][d] (MN-major)
+    Operand A{dlogits, ldv, N * ldv, V, N, dt, false};
+    Operand Bw{w_op, ld_w, V * ld_w, D, V, dt, true};
+    GemmShape s{1, (int)N, (int)D, (int)V, CAUSAL_NONE};
+    if (int rc = run_gemm(A, Bw, s, make_epilogue(EPI_STORE, dh_dtype, dh, D, N * D, nullptr), st)) return rc;
+  }
+  if (!dw) return ULM_OK;
+  // dW = dx^T h: A = dx as [row][token] (MN-major), B = h as [row][d] (MN-major)
+  Operand A{dlogits, ldv, N * ldv, V, N, dt, true};
+  Operand Bh{h_op, ld_h, N * ld_h, D, N, dt, true};
+  GemmShape s{1, (int)V, (int)D, (int)N, CAUSAL_NONE};
+  return run_gemm(A, Bh, s, make_epilogue(EPI_STORE, dw_dtype, dw, D, V * D, nullptr), st);
+}

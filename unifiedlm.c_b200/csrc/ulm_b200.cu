@@ -7,3 +7,6 @@
 #include "address.cu"
 #include "head.cu"
 #include "norm.cu"
+#include "logprobs.cu"
+#include "embed.cu"
+#include "clip.cu"

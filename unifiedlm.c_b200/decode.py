@@ -20,6 +20,7 @@ import math
 import torch
 
 from . import _lib as L
+from .logprobs import token_logprobs
 
 
 def rmsnorm_rows(x, weight, eps):
@@ -179,6 +180,13 @@ class BatchedDecoder:
         greedy at temperature 0)."""
         self._run_step(sample=True)
         return self.next_token
+
+    def logprobs(self, tokens=None, top_k=0):
+        """`logprobs.TokenLogprobs` (B,) under the last step's logits: of `tokens` (B,), by default the
+        tokens that the step chose, with the entropies and the top_k best alternatives (at temperature
+        1, whatever the sampler's)."""
+        tokens = self.next_token if tokens is None else tokens.to(self.dev)
+        return token_logprobs(self.logits, tokens, top_k=top_k)
 
     def prepare_graph(self):
         """Capture the step graphs (each runs the step on scratch state), then reset."""

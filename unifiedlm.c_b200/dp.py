@@ -15,6 +15,8 @@ one-shot `all_reduce`.
 import torch
 import torch.distributed as dist
 
+from .clip import clip_grads
+
 
 class GradBucket:
     def __init__(self, shapes, device, dtype=torch.float32, segments=1):
@@ -41,6 +43,16 @@ class GradBucket:
         else:
             torch.cat([g.reshape(-1).to(self.flat.dtype) for g in grads], out=self.flat)
         return self.flat
+
+    def pack_clipped(self, grads, max_norm):
+        """`pack` and clip in one pass, where no ranks are to be averaged in between: the bucket holds
+        the gradients scaled to a 2-norm of at most `max_norm`. Returns the norm that they had."""
+        return clip_grads(grads, max_norm, out=self.views())
+
+    def clip_norm_(self, max_norm):
+        """Scale the packed (and averaged) gradients to a 2-norm of at most `max_norm` in place. Returns
+        the norm that they had; after an all-reduce it is the same on every rank."""
+        return clip_grads([self.flat], max_norm)
 
     def _segment_range(self, i):
         if not 0 <= i < self.segments:

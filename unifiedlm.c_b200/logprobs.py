@@ -1,0 +1,246 @@
+"""Log probabilities of given tokens on sm_100a, with the entropy and the best alternatives.
+
+For logits x of a row and its token t (the log_softmax and gather that score a text, a policy's
+samples or a decode step; the reference's logits are model.py:153-157):
+
+    logprob = x_t - logsumexp(x),   entropy = - sum_v p_v log p_v,   p = softmax(x)
+
+and the `top_k` best tokens in descending order (the lower id first among equals).
+
+`lm_head_logprobs(h, weight, tokens)` takes the logits h @ weight.T of the output Linear, like
+`head.lm_head_loss`; `token_logprobs(logits, tokens)` takes logits that exist already (a decode
+step's, `BatchedDecoder.logprobs`). Both are differentiable in logprobs and entropy. Token -1 is
+padding: logprob 0, no gradient through it. Any other token outside the vocabulary makes its
+logprob, and the gradients that it reaches, NaN. Masked tokens (logits of -inf) have probability 0;
+a row that is masked throughout, or holds a NaN or +inf, has NaN results, as log_softmax has. The
+work runs in libulm_b200.so (ulm_lm_head_logprobs_*, ulm_token_logprobs_*) through `torch.library`
+ops. No CPU path.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib as L
+from .kernel import PRECISION, _op_dtype, operand_ld
+
+MAX_TOP_K = 32
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # (...) fp32
+    entropy: torch.Tensor       # (...) fp32
+    top_ids: torch.Tensor       # (..., top_k) int64
+    top_logprobs: torch.Tensor  # (..., top_k) fp32
+
+
+def _operand(x, opt):
+    """(matrix, row stride) of a 2-d operand of a product: x itself where it can be read in place, else
+    a padded copy in the operand type."""
+    n, d = x.shape
+    ld = x.stride(0) if n > 1 else operand_ld(d)
+    if (x.dtype == opt and (d == 1 or x.stride(1) == 1) and ld >= d and
+            (opt == torch.float32 or (ld % 8 == 0 and x.data_ptr() % 16 == 0))):
+        return x, ld
+    c = torch.empty(n, operand_ld(d), device=x.device, dtype=opt)
+    c[:, :d] = x
+    return c, operand_ld(d)
+
+
+def _outputs(N, top_k, dev):
+    f32 = dict(device=dev, dtype=torch.float32)
+    return (torch.empty(N, **f32), torch.empty(N, **f32), torch.empty(N, 2, **f32),
+            torch.empty(N, top_k, device=dev, dtype=torch.int64), torch.empty(N, top_k, **f32))
+
+
+_OUT = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+
+
+# ---- from hidden states -------------------------------------------------------------------------------
+
+@torch.library.custom_op("ulm::lm_head_logprobs_fwd", mutates_args=())
+def lm_head_logprobs_fwd(h: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, top_k: int, precision: int) -> _OUT:
+    """h (N, D), weight (V, D), tokens (N,) int64. Returns (logprobs, entropy, stats, top_ids,
+    top_logprobs); stats (N, 2) is saved for the backward."""
+    N, D = h.shape
+    V = weight.shape[0]
+    lp, ent, stats, ids, tlp = _outputs(N, top_k, h.device)
+    opt = _op_dtype(precision)
+    h_op, ld_h = _operand(h.detach(), opt)
+    w_op, ld_w = _operand(weight.detach(), opt)
+    work = torch.empty(int(L.lib().ulm_lm_head_logprobs_work_bytes(N, V, D, 0, precision)), device=h.device,
+                       dtype=torch.uint8)
+    with torch.cuda.device(h.device):
+        L.check(L.lib().ulm_lm_head_logprobs_fwd(L.ptr(h_op), ld_h, L.ptr(w_op), ld_w, L.ptr(tokens), L.ptr(lp),
+                                                 L.ptr(ent), L.ptr(stats), L.ptr(ids), L.ptr(tlp), L.ptr(work), N, V, D,
+                                                 top_k, precision, L.stream_of(h)))
+    return lp, ent, stats, ids, tlp
+
+
+@lm_head_logprobs_fwd.register_fake
+def _lm_head_logprobs_fwd_fake(h, weight, tokens, top_k, precision):
+    return _outputs(h.shape[0], top_k, h.device)
+
+
+@torch.library.custom_op("ulm::lm_head_logprobs_bwd", mutates_args=())
+def lm_head_logprobs_bwd(dlp: Optional[torch.Tensor], dent: Optional[torch.Tensor], h: torch.Tensor,
+                         weight: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor, ent: torch.Tensor,
+                         precision: int, need_dh: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Returns (dh in h's type, dweight in weight's type); one that is not needed is empty."""
+    N, D = h.shape
+    V = weight.shape[0]
+    dh, dw = _lm_head_logprobs_bwd_fake(dlp, dent, h, weight, tokens, stats, ent, precision, need_dh, need_dw)
+    opt = _op_dtype(precision)
+    h_op, ld_h = _operand(h.detach(), opt)
+    w_op, ld_w = _operand(weight.detach(), opt)
+    work = torch.empty(int(L.lib().ulm_lm_head_logprobs_work_bytes(N, V, D, 1, precision)), device=h.device,
+                       dtype=torch.uint8)
+    with torch.cuda.device(h.device):
+        L.check(L.lib().ulm_lm_head_logprobs_bwd(
+            L.ptr(dlp), L.ptr(dent), L.ptr(h_op), ld_h, L.ptr(w_op), ld_w, L.ptr(tokens), L.ptr(stats), L.ptr(ent),
+            L.ptr(dh) if need_dh else None, L.dtype_code(dh.dtype), L.ptr(dw) if need_dw else None,
+            L.dtype_code(dw.dtype), L.ptr(work), N, V, D, precision, L.stream_of(h)))
+    return dh, dw
+
+
+@lm_head_logprobs_bwd.register_fake
+def _lm_head_logprobs_bwd_fake(dlp, dent, h, weight, tokens, stats, ent, precision, need_dh, need_dw):
+    return (torch.empty(h.shape if need_dh else (0,), device=h.device, dtype=h.dtype),
+            torch.empty(weight.shape if need_dw else (0,), device=h.device, dtype=weight.dtype))
+
+
+def _head_setup(ctx, inputs, output):
+    h, weight, tokens, top_k, precision = inputs
+    _, ent, stats, ids, tlp = output
+    ctx.save_for_backward(h, weight, tokens, stats, ent)
+    ctx.precision = precision
+    ctx.mark_non_differentiable(stats, ids, tlp)
+    ctx.set_materialize_grads(False)
+
+
+def _grad_in(g):
+    return None if g is None else g.float().contiguous()
+
+
+def _head_backward(ctx, dlp, dent, *unused):
+    if dlp is None and dent is None:
+        return (None,) * 5
+    h, weight, tokens, stats, ent = ctx.saved_tensors
+    need_dh, need_dw = ctx.needs_input_grad[:2]
+    dh, dw = lm_head_logprobs_bwd(_grad_in(dlp), _grad_in(dent), h, weight, tokens, stats, ent, ctx.precision,
+                                  need_dh, need_dw)
+    return dh if need_dh else None, dw if need_dw else None, None, None, None
+
+
+torch.library.register_autograd("ulm::lm_head_logprobs_fwd", _head_backward, setup_context=_head_setup)
+
+
+# ---- from logits --------------------------------------------------------------------------------------
+
+def _row_stride(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+@torch.library.custom_op("ulm::token_logprobs_fwd", mutates_args=())
+def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top_k: int) -> _OUT:
+    """logits (N, V), tokens (N,) int64; the outputs of lm_head_logprobs_fwd."""
+    N, V = logits.shape
+    lp, ent, stats, ids, tlp = _outputs(N, top_k, logits.device)
+    with torch.cuda.device(logits.device):
+        L.check(L.lib().ulm_token_logprobs_fwd(L.ptr(logits), L.dtype_code(logits.dtype), _row_stride(logits),
+                                               L.ptr(tokens), L.ptr(lp), L.ptr(ent), L.ptr(stats), L.ptr(ids),
+                                               L.ptr(tlp), N, V, top_k, L.stream_of(logits)))
+    return lp, ent, stats, ids, tlp
+
+
+@token_logprobs_fwd.register_fake
+def _token_logprobs_fwd_fake(logits, tokens, top_k):
+    return _outputs(logits.shape[0], top_k, logits.device)
+
+
+@torch.library.custom_op("ulm::token_logprobs_bwd", mutates_args=())
+def token_logprobs_bwd(dlp: Optional[torch.Tensor], dent: Optional[torch.Tensor], logits: torch.Tensor,
+                       tokens: torch.Tensor, stats: torch.Tensor, ent: torch.Tensor) -> torch.Tensor:
+    """Returns dlogits (N, V) in logits' type."""
+    N, V = logits.shape
+    d = torch.empty(N, V, device=logits.device, dtype=logits.dtype)
+    with torch.cuda.device(logits.device):
+        L.check(L.lib().ulm_token_logprobs_bwd(L.ptr(dlp), L.ptr(dent), L.ptr(logits), L.dtype_code(logits.dtype),
+                                               _row_stride(logits), L.ptr(tokens), L.ptr(stats), L.ptr(ent), L.ptr(d), V,
+                                               N, V, L.stream_of(logits)))
+    return d
+
+
+@token_logprobs_bwd.register_fake
+def _token_logprobs_bwd_fake(dlp, dent, logits, tokens, stats, ent):
+    return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+
+
+def _logits_setup(ctx, inputs, output):
+    logits, tokens, top_k = inputs
+    _, ent, stats, ids, tlp = output
+    ctx.save_for_backward(logits, tokens, stats, ent)
+    ctx.mark_non_differentiable(stats, ids, tlp)
+    ctx.set_materialize_grads(False)
+
+
+def _logits_backward(ctx, dlp, dent, *unused):
+    if dlp is None and dent is None:
+        return None, None, None
+    logits, tokens, stats, ent = ctx.saved_tensors
+    return token_logprobs_bwd(_grad_in(dlp), _grad_in(dent), logits, tokens, stats, ent), None, None
+
+
+torch.library.register_autograd("ulm::token_logprobs_fwd", _logits_backward, setup_context=_logits_setup)
+
+
+# ---- entry points -------------------------------------------------------------------------------------
+
+def _check(x, tokens, V, top_k, name):
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU path)")
+    if x.dim() < 1 or tokens.shape != x.shape[:-1]:
+        raise ValueError(f"tokens {tuple(tokens.shape)} do not match the rows of {tuple(x.shape)}")
+    if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+        raise TypeError(f"tokens must be integers, got {tokens.dtype}")
+    if tokens.device != x.device:
+        raise ValueError(f"tokens on {tokens.device}, {x.device} expected")
+    if V < 1:
+        raise ValueError("empty vocabulary")
+    if not 0 <= top_k <= min(V, MAX_TOP_K):
+        raise ValueError(f"top_k={top_k} must be in 0 .. min(vocabulary, {MAX_TOP_K})")
+
+
+def _shaped(out, shape, top_k):
+    lp, ent, _, ids, tlp = out
+    return TokenLogprobs(lp.view(shape), ent.view(shape), ids.view(*shape, top_k), tlp.view(*shape, top_k))
+
+
+def lm_head_logprobs(h, weight, tokens, top_k=0, precision="bf16"):
+    """TokenLogprobs of `tokens` (...) under the logits h @ weight.T: h (..., D) fp32 or bf16, weight
+    (V, D) fp32 or bf16. "bf16" contracts bf16 operands (rounding fp32 ones), "fp32" fp32 ones; the
+    statistics are fp32. Gradients of h and weight flow from logprobs and entropy, in the types of h
+    and weight; the alternatives are not differentiable."""
+    if weight.dim() != 2 or h.dim() < 1 or h.shape[-1] != weight.shape[1]:
+        raise ValueError(f"h {tuple(h.shape)} and weight {tuple(weight.shape)} do not match")
+    if precision not in PRECISION:
+        raise ValueError(f"precision must be one of {sorted(PRECISION)}, got {precision!r}")
+    _check(h, tokens, weight.shape[0], top_k, "lm_head_logprobs")
+    if weight.device != h.device:
+        raise ValueError(f"weight on {weight.device}, {h.device} expected")
+    hh = h.reshape(-1, h.shape[-1])
+    hh = hh if hh.dtype in (torch.float32, torch.bfloat16) else hh.float()
+    ww = weight if weight.dtype in (torch.float32, torch.bfloat16) else weight.float()
+    tk = tokens.reshape(-1).to(torch.int64).contiguous()
+    out = torch.ops.ulm.lm_head_logprobs_fwd(hh, ww, tk, top_k, PRECISION[precision])
+    return _shaped(out, tokens.shape, top_k)
+
+
+def token_logprobs(logits, tokens, top_k=0):
+    """TokenLogprobs of `tokens` (...) under `logits` (..., V) fp32 or bf16."""
+    _check(logits, tokens, logits.shape[-1] if logits.dim() else 0, top_k, "token_logprobs")
+    x = logits.reshape(-1, logits.shape[-1])
+    x = x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    tk = tokens.reshape(-1).to(torch.int64).contiguous()
+    return _shaped(torch.ops.ulm.token_logprobs_fwd(x, tk, top_k), tokens.shape, top_k)

@@ -13,7 +13,10 @@ libulm_b200.so:
 * UnifiedBlock.init_state / step (model.py:88-111) and UnifiedLM.forward_recurrent (:164-175): the
   batched decode kernels (ulm_decode_*), the same state dict (buf, U, c, r_prev) kept in fp32.
 * UnifiedLM.forward with `fused_head`: output Linear + cross entropy without the logits
-  (`head.lm_head_loss`).
+  (`head.lm_head_loss`); with `fused_embedding`: the token embedding and its gradient
+  (`embed.embedding`).
+* UnifiedLM.token_logprobs: log probabilities of given tokens, entropies and the best alternatives
+  without the logits (`logprobs.lm_head_logprobs`).
 
 `UnifiedBlock.precision` ("bf16" tensor-core products, default; "fp32" for the 1e-5 parity mode) is
 set for a whole model by `UnifiedLM.set_precision`.
@@ -29,8 +32,10 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .block import addressed_memory, block_scalars, unified_block
+from .embed import embedding
 from .head import lm_head_loss
 from .kernel import CHUNK
+from .logprobs import lm_head_logprobs
 from .norm import linear, rms_norm
 
 
@@ -201,6 +206,8 @@ class UnifiedLM(nn.Module):
         # True: forward(tokens, targets) computes last_loss with the fused head and returns None
         # instead of the logits (training loops that only read last_loss, as train.py does)
         self.fused_head = False
+        # True: the token embedding and its gradient run in the library (`embed.embedding`)
+        self.fused_embedding = False
 
     @torch.no_grad()
     def _reset_parameters(self):
@@ -223,11 +230,23 @@ class UnifiedLM(nn.Module):
             layer.precision = precision
         return self
 
-    def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None) -> torch.Tensor:
-        h = self.dropout(self.tok_embeddings(tokens))
+    def _hidden(self, tokens):
+        """The final-normed hidden states (B, T, d)."""
+        h = embedding(tokens, self.tok_embeddings.weight) if self.fused_embedding else self.tok_embeddings(tokens)
+        h = self.dropout(h)
         for layer in self.layers:
             h = layer(h)
-        h = self.norm(h)
+        return self.norm(h)
+
+    def token_logprobs(self, tokens: torch.Tensor, targets: torch.Tensor, top_k: int = 0):
+        """`logprobs.TokenLogprobs` of `targets` (B, T) after every position of `tokens` (B, T), without
+        the (B, T, V) logits: log probabilities and entropies with gradients, and the top_k best
+        alternatives. Targets of -1 are padding."""
+        prec = self.layers[0].precision if len(self.layers) else "bf16"
+        return lm_head_logprobs(self._hidden(tokens), self.output.weight, targets, top_k=top_k, precision=prec)
+
+    def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        h = self._hidden(tokens)
         if targets is None:
             self.last_loss = None
             return self.output(h[:, [-1], :])
