@@ -140,3 +140,33 @@ def device_error():
     site = _I(0)
     check(lib().ulm_device_error(ctypes.byref(site)))
     return site.value
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def eager(*ts):
+    """Whether the tensors hold data that a call can read now (nothing is traced, compiled or faked): the
+    entries then call the library directly, without the dispatcher's cost of a custom op."""
+    if torch.compiler.is_compiling():
+        return False
+    for t in ts:
+        if type(t) not in _PLAIN:
+            return False
+    return True
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(device):
+    """`torch.cuda.device(device)`, or nothing where it is the current one already."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)

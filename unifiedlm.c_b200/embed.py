@@ -11,17 +11,54 @@ import torch
 from . import _lib as L
 
 
+def embedding_fwd_raw(tokens, weight, scale, out_bf16):
+    """ulm_embedding_fwd on a fresh buffer: y (N, D)."""
+    N = tokens.shape[0]
+    V, D = weight.shape
+    dt = torch.bfloat16 if out_bf16 else weight.dtype
+    y = torch.empty(N, D, device=weight.device, dtype=dt)
+    with L.on(weight.device):
+        L.check(L.lib().ulm_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), L.dtype_code(weight.dtype),
+                                          weight.stride(0) if V > 1 else D, y.data_ptr(), L.dtype_code(dt), N, V, D,
+                                          scale, L.stream_of(weight)))
+    return y
+
+
+def embedding_bwd_raw(tokens, dy, V, scale, dw_bf16):
+    """ulm_embedding_bwd on a fresh buffer: dweight (V, D)."""
+    N, D = dy.shape
+    dt = torch.bfloat16 if dw_bf16 else torch.float32
+    lib = L.lib()
+    dw = torch.empty(V, D, device=dy.device, dtype=dt)
+    work = torch.empty(lib.ulm_embedding_bwd_work_bytes(N, V, D), device=dy.device, dtype=torch.uint8)
+    with L.on(dy.device):
+        L.check(lib.ulm_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), L.dtype_code(dy.dtype), dw.data_ptr(),
+                                      L.dtype_code(dt), work.data_ptr(), N, V, D, scale, L.stream_of(dy)))
+    return dw
+
+
+class _Embedding(torch.autograd.Function):
+    """The eager form of the two ops below."""
+
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, out_bf16):
+        ctx.save_for_backward(tokens)
+        ctx.meta = (weight.shape[0], scale, weight.dtype == torch.bfloat16)
+        ctx.set_materialize_grads(False)
+        return embedding_fwd_raw(tokens, weight, scale, out_bf16)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        if dy is None:
+            return None, None, None, None
+        return None, embedding_bwd_raw(*ctx.saved_tensors, dy.contiguous(), *ctx.meta), None, None
+
+
 @torch.library.custom_op("ulm::embedding_fwd", mutates_args=())
 def embedding_fwd(tokens: torch.Tensor, weight: torch.Tensor, scale: float, out_bf16: bool) -> torch.Tensor:
     """tokens (N,) int64, weight (V, D); y (N, D) in weight's type, or bf16 (out_bf16)."""
-    N = tokens.shape[0]
-    V, D = weight.shape
-    y = _embedding_fwd_fake(tokens, weight, scale, out_bf16)
-    ld = weight.stride(0) if V > 1 else D
-    with torch.cuda.device(weight.device):
-        L.check(L.lib().ulm_embedding_fwd(L.ptr(tokens), L.ptr(weight), L.dtype_code(weight.dtype), ld, L.ptr(y),
-                                          L.dtype_code(y.dtype), N, V, D, scale, L.stream_of(weight)))
-    return y
+    return embedding_fwd_raw(tokens, weight, scale, out_bf16)
 
 
 @embedding_fwd.register_fake
@@ -33,13 +70,7 @@ def _embedding_fwd_fake(tokens, weight, scale, out_bf16):
 @torch.library.custom_op("ulm::embedding_bwd", mutates_args=())
 def embedding_bwd(tokens: torch.Tensor, dy: torch.Tensor, V: int, scale: float, dw_bf16: bool) -> torch.Tensor:
     """dweight (V, D), fp32 or bf16, of dy (N, D)."""
-    N, D = dy.shape
-    dw = _embedding_bwd_fake(tokens, dy, V, scale, dw_bf16)
-    work = torch.empty(int(L.lib().ulm_embedding_bwd_work_bytes(N, V, D)), device=dy.device, dtype=torch.uint8)
-    with torch.cuda.device(dy.device):
-        L.check(L.lib().ulm_embedding_bwd(L.ptr(tokens), L.ptr(dy), L.dtype_code(dy.dtype), L.ptr(dw),
-                                          L.dtype_code(dw.dtype), L.ptr(work), N, V, D, scale, L.stream_of(dy)))
-    return dw
+    return embedding_bwd_raw(tokens, dy, V, scale, dw_bf16)
 
 
 @embedding_bwd.register_fake
@@ -84,6 +115,13 @@ def embedding(tokens, weight, scale=1.0, out_dtype=None):
     w = weight
     if D > 1 and w.stride(1) != 1 or V > 1 and w.stride(0) < D:
         w = w.contiguous()
-    tk = tokens.reshape(-1).to(torch.int64).contiguous()
-    y = torch.ops.ulm.embedding_fwd(tk, w, float(scale), out_dtype == torch.bfloat16)
-    return y.view(*tokens.shape, D)
+    tk = tokens if tokens.dim() == 1 else tokens.reshape(-1)
+    tk = tk.to(torch.int64).contiguous()
+    args = tk, w, float(scale), out_dtype == torch.bfloat16
+    if not L.eager(tk, w):
+        y = torch.ops.ulm.embedding_fwd(*args)
+    elif w.requires_grad and torch.is_grad_enabled():
+        y = _Embedding.apply(*args)
+    else:
+        y = embedding_fwd_raw(*args)
+    return y if tokens.dim() == 1 else y.view(*tokens.shape, D)

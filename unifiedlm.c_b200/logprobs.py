@@ -46,10 +46,14 @@ def _operand(x, opt):
     return c, operand_ld(d)
 
 
-def _outputs(N, top_k, dev):
+def _outputs(N, top_k, dev, stats=True):
     f32 = dict(device=dev, dtype=torch.float32)
-    return (torch.empty(N, **f32), torch.empty(N, **f32), torch.empty(N, 2, **f32),
+    return (torch.empty(N, **f32), torch.empty(N, **f32), torch.empty(N, 2, **f32) if stats else None,
             torch.empty(N, top_k, device=dev, dtype=torch.int64), torch.empty(N, top_k, **f32))
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 _OUT = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
@@ -57,23 +61,74 @@ _OUT = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tenso
 
 # ---- from hidden states -------------------------------------------------------------------------------
 
+def lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision, stats=True):
+    """ulm_lm_head_logprobs_fwd on fresh buffers: (logprobs, entropy, stats or None, top_ids,
+    top_logprobs)."""
+    N, D = h.shape
+    V = weight.shape[0]
+    lib = L.lib()
+    out = lp, ent, st, ids, tlp = _outputs(N, top_k, h.device, stats)
+    opt = _op_dtype(precision)
+    h_op, ld_h = _operand(h.detach(), opt)
+    w_op, ld_w = _operand(weight.detach(), opt)
+    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, precision), device=h.device, dtype=torch.uint8)
+    with L.on(h.device):
+        L.check(lib.ulm_lm_head_logprobs_fwd(h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(),
+                                             lp.data_ptr(), ent.data_ptr(), _addr(st), ids.data_ptr(), tlp.data_ptr(),
+                                             work.data_ptr(), N, V, D, top_k, precision, L.stream_of(h)))
+    return out
+
+
+def lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision, need_dh, need_dw):
+    """ulm_lm_head_logprobs_bwd on fresh buffers: (dh, dweight), None for one that is not needed."""
+    N, D = h.shape
+    V = weight.shape[0]
+    lib = L.lib()
+    dh = torch.empty(N, D, device=h.device, dtype=h.dtype) if need_dh else None
+    dw = torch.empty(V, D, device=h.device, dtype=weight.dtype) if need_dw else None
+    opt = _op_dtype(precision)
+    h_op, ld_h = _operand(h.detach(), opt)
+    w_op, ld_w = _operand(weight.detach(), opt)
+    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 1, precision), device=h.device, dtype=torch.uint8)
+    with L.on(h.device):
+        L.check(lib.ulm_lm_head_logprobs_bwd(
+            _addr(dlp), _addr(dent), h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(), stats.data_ptr(),
+            ent.data_ptr(), _addr(dh), L.dtype_code(h.dtype), _addr(dw), L.dtype_code(weight.dtype), work.data_ptr(),
+            N, V, D, precision, L.stream_of(h)))
+    return dh, dw
+
+
+def _grad_in(g):
+    return None if g is None else g.float().contiguous()
+
+
+class _HeadLogprobs(torch.autograd.Function):
+    """The eager form of the two ops below."""
+
+    @staticmethod
+    def forward(ctx, h, weight, tokens, top_k, precision):
+        lp, ent, stats, ids, tlp = lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision)
+        ctx.save_for_backward(h, weight, tokens, stats, ent)
+        ctx.precision = precision
+        ctx.mark_non_differentiable(ids, tlp)
+        ctx.set_materialize_grads(False)
+        return lp, ent, ids, tlp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlp, dent, *unused):
+        if dlp is None and dent is None:
+            return None, None, None, None, None
+        dh, dw = lm_head_logprobs_bwd_raw(_grad_in(dlp), _grad_in(dent), *ctx.saved_tensors, ctx.precision,
+                                          *ctx.needs_input_grad[:2])
+        return dh, dw, None, None, None
+
+
 @torch.library.custom_op("ulm::lm_head_logprobs_fwd", mutates_args=())
 def lm_head_logprobs_fwd(h: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, top_k: int, precision: int) -> _OUT:
     """h (N, D), weight (V, D), tokens (N,) int64. Returns (logprobs, entropy, stats, top_ids,
     top_logprobs); stats (N, 2) is saved for the backward."""
-    N, D = h.shape
-    V = weight.shape[0]
-    lp, ent, stats, ids, tlp = _outputs(N, top_k, h.device)
-    opt = _op_dtype(precision)
-    h_op, ld_h = _operand(h.detach(), opt)
-    w_op, ld_w = _operand(weight.detach(), opt)
-    work = torch.empty(int(L.lib().ulm_lm_head_logprobs_work_bytes(N, V, D, 0, precision)), device=h.device,
-                       dtype=torch.uint8)
-    with torch.cuda.device(h.device):
-        L.check(L.lib().ulm_lm_head_logprobs_fwd(L.ptr(h_op), ld_h, L.ptr(w_op), ld_w, L.ptr(tokens), L.ptr(lp),
-                                                 L.ptr(ent), L.ptr(stats), L.ptr(ids), L.ptr(tlp), L.ptr(work), N, V, D,
-                                                 top_k, precision, L.stream_of(h)))
-    return lp, ent, stats, ids, tlp
+    return lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision)
 
 
 @lm_head_logprobs_fwd.register_fake
@@ -86,20 +141,8 @@ def lm_head_logprobs_bwd(dlp: Optional[torch.Tensor], dent: Optional[torch.Tenso
                          weight: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor, ent: torch.Tensor,
                          precision: int, need_dh: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """Returns (dh in h's type, dweight in weight's type); one that is not needed is empty."""
-    N, D = h.shape
-    V = weight.shape[0]
-    dh, dw = _lm_head_logprobs_bwd_fake(dlp, dent, h, weight, tokens, stats, ent, precision, need_dh, need_dw)
-    opt = _op_dtype(precision)
-    h_op, ld_h = _operand(h.detach(), opt)
-    w_op, ld_w = _operand(weight.detach(), opt)
-    work = torch.empty(int(L.lib().ulm_lm_head_logprobs_work_bytes(N, V, D, 1, precision)), device=h.device,
-                       dtype=torch.uint8)
-    with torch.cuda.device(h.device):
-        L.check(L.lib().ulm_lm_head_logprobs_bwd(
-            L.ptr(dlp), L.ptr(dent), L.ptr(h_op), ld_h, L.ptr(w_op), ld_w, L.ptr(tokens), L.ptr(stats), L.ptr(ent),
-            L.ptr(dh) if need_dh else None, L.dtype_code(dh.dtype), L.ptr(dw) if need_dw else None,
-            L.dtype_code(dw.dtype), L.ptr(work), N, V, D, precision, L.stream_of(h)))
-    return dh, dw
+    dh, dw = lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision, need_dh, need_dw)
+    return h.new_empty(0) if dh is None else dh, weight.new_empty(0) if dw is None else dw
 
 
 @lm_head_logprobs_bwd.register_fake
@@ -115,10 +158,6 @@ def _head_setup(ctx, inputs, output):
     ctx.precision = precision
     ctx.mark_non_differentiable(stats, ids, tlp)
     ctx.set_materialize_grads(False)
-
-
-def _grad_in(g):
-    return None if g is None else g.float().contiguous()
 
 
 def _head_backward(ctx, dlp, dent, *unused):
@@ -140,16 +179,51 @@ def _row_stride(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def token_logprobs_fwd_raw(logits, tokens, top_k, stats=True):
+    """ulm_token_logprobs_fwd on fresh buffers, as lm_head_logprobs_fwd_raw."""
+    N, V = logits.shape
+    out = lp, ent, st, ids, tlp = _outputs(N, top_k, logits.device, stats)
+    with L.on(logits.device):
+        L.check(L.lib().ulm_token_logprobs_fwd(logits.data_ptr(), L.dtype_code(logits.dtype), _row_stride(logits),
+                                               tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), _addr(st),
+                                               ids.data_ptr(), tlp.data_ptr(), N, V, top_k, L.stream_of(logits)))
+    return out
+
+
+def token_logprobs_bwd_raw(dlp, dent, logits, tokens, stats, ent):
+    """ulm_token_logprobs_bwd on a fresh buffer: dlogits (N, V) in logits' type."""
+    N, V = logits.shape
+    d = torch.empty(N, V, device=logits.device, dtype=logits.dtype)
+    with L.on(logits.device):
+        L.check(L.lib().ulm_token_logprobs_bwd(_addr(dlp), _addr(dent), logits.data_ptr(), L.dtype_code(logits.dtype),
+                                               _row_stride(logits), tokens.data_ptr(), stats.data_ptr(), ent.data_ptr(),
+                                               d.data_ptr(), V, N, V, L.stream_of(logits)))
+    return d
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """The eager form of the two ops below."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k):
+        lp, ent, stats, ids, tlp = token_logprobs_fwd_raw(logits, tokens, top_k)
+        ctx.save_for_backward(logits, tokens, stats, ent)
+        ctx.mark_non_differentiable(ids, tlp)
+        ctx.set_materialize_grads(False)
+        return lp, ent, ids, tlp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlp, dent, *unused):
+        if dlp is None and dent is None:
+            return None, None, None
+        return token_logprobs_bwd_raw(_grad_in(dlp), _grad_in(dent), *ctx.saved_tensors), None, None
+
+
 @torch.library.custom_op("ulm::token_logprobs_fwd", mutates_args=())
 def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top_k: int) -> _OUT:
     """logits (N, V), tokens (N,) int64; the outputs of lm_head_logprobs_fwd."""
-    N, V = logits.shape
-    lp, ent, stats, ids, tlp = _outputs(N, top_k, logits.device)
-    with torch.cuda.device(logits.device):
-        L.check(L.lib().ulm_token_logprobs_fwd(L.ptr(logits), L.dtype_code(logits.dtype), _row_stride(logits),
-                                               L.ptr(tokens), L.ptr(lp), L.ptr(ent), L.ptr(stats), L.ptr(ids),
-                                               L.ptr(tlp), N, V, top_k, L.stream_of(logits)))
-    return lp, ent, stats, ids, tlp
+    return token_logprobs_fwd_raw(logits, tokens, top_k)
 
 
 @token_logprobs_fwd.register_fake
@@ -161,13 +235,7 @@ def _token_logprobs_fwd_fake(logits, tokens, top_k):
 def token_logprobs_bwd(dlp: Optional[torch.Tensor], dent: Optional[torch.Tensor], logits: torch.Tensor,
                        tokens: torch.Tensor, stats: torch.Tensor, ent: torch.Tensor) -> torch.Tensor:
     """Returns dlogits (N, V) in logits' type."""
-    N, V = logits.shape
-    d = torch.empty(N, V, device=logits.device, dtype=logits.dtype)
-    with torch.cuda.device(logits.device):
-        L.check(L.lib().ulm_token_logprobs_bwd(L.ptr(dlp), L.ptr(dent), L.ptr(logits), L.dtype_code(logits.dtype),
-                                               _row_stride(logits), L.ptr(tokens), L.ptr(stats), L.ptr(ent), L.ptr(d), V,
-                                               N, V, L.stream_of(logits)))
-    return d
+    return token_logprobs_bwd_raw(dlp, dent, logits, tokens, stats, ent)
 
 
 @token_logprobs_bwd.register_fake
@@ -210,8 +278,16 @@ def _check(x, tokens, V, top_k, name):
         raise ValueError(f"top_k={top_k} must be in 0 .. min(vocabulary, {MAX_TOP_K})")
 
 
+def _rows(t):
+    """tokens as one int64 row"""
+    t = t if t.dim() == 1 else t.reshape(-1)
+    return t.to(torch.int64).contiguous()
+
+
 def _shaped(out, shape, top_k):
-    lp, ent, _, ids, tlp = out
+    lp, ent, ids, tlp = out[0], out[1], out[-2], out[-1]
+    if len(shape) == 1:
+        return TokenLogprobs(lp, ent, ids, tlp)
     return TokenLogprobs(lp.view(shape), ent.view(shape), ids.view(*shape, top_k), tlp.view(*shape, top_k))
 
 
@@ -227,20 +303,31 @@ def lm_head_logprobs(h, weight, tokens, top_k=0, precision="bf16"):
     _check(h, tokens, weight.shape[0], top_k, "lm_head_logprobs")
     if weight.device != h.device:
         raise ValueError(f"weight on {weight.device}, {h.device} expected")
-    hh = h.reshape(-1, h.shape[-1])
+    hh = h if h.dim() == 2 else h.reshape(-1, h.shape[-1])
     hh = hh if hh.dtype in (torch.float32, torch.bfloat16) else hh.float()
     ww = weight if weight.dtype in (torch.float32, torch.bfloat16) else weight.float()
-    tk = tokens.reshape(-1).to(torch.int64).contiguous()
-    out = torch.ops.ulm.lm_head_logprobs_fwd(hh, ww, tk, top_k, PRECISION[precision])
+    args = hh, ww, _rows(tokens), top_k, PRECISION[precision]
+    if not L.eager(hh, ww, tokens):
+        out = torch.ops.ulm.lm_head_logprobs_fwd(*args)
+    elif (hh.requires_grad or ww.requires_grad) and torch.is_grad_enabled():
+        out = _HeadLogprobs.apply(*args)
+    else:
+        out = lm_head_logprobs_fwd_raw(*args, stats=False)
     return _shaped(out, tokens.shape, top_k)
 
 
 def token_logprobs(logits, tokens, top_k=0):
     """TokenLogprobs of `tokens` (...) under `logits` (..., V) fp32 or bf16."""
     _check(logits, tokens, logits.shape[-1] if logits.dim() else 0, top_k, "token_logprobs")
-    x = logits.reshape(-1, logits.shape[-1])
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     x = x if x.dtype in (torch.float32, torch.bfloat16) else x.float()
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()
-    tk = tokens.reshape(-1).to(torch.int64).contiguous()
-    return _shaped(torch.ops.ulm.token_logprobs_fwd(x, tk, top_k), tokens.shape, top_k)
+    tk = _rows(tokens)
+    if not L.eager(x, tokens):
+        out = torch.ops.ulm.token_logprobs_fwd(x, tk, top_k)
+    elif x.requires_grad and torch.is_grad_enabled():
+        out = _TokenLogprobs.apply(x, tk, top_k)
+    else:
+        out = token_logprobs_fwd_raw(x, tk, top_k, stats=False)
+    return _shaped(out, tokens.shape, top_k)
