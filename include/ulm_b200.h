@@ -461,18 +461,18 @@ int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const 
                            int64_t N, int64_t V, void* stream);
 
 /* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd.
- * work: ulm_lm_head_logprobs_work_bytes(N,V,D,0,prec) bytes. */
+ * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 256-byte aligned. */
 int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens,
                              float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
                              void* work, int64_t N, int64_t V, int64_t D, int top_k, int prec, void* stream);
 /* Backward: dh (N,D) of dh_dtype and dw (V,D) of dw_dtype (either may be NULL: not wanted); the logits
  * are recomputed. work:
- * ulm_lm_head_logprobs_work_bytes(N,V,D,1,prec) bytes. */
+ * ulm_lm_head_logprobs_work_bytes(N,V,D,0,1,prec) bytes, 256-byte aligned. */
 int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
                              const void* w_op, int64_t ld_w, const int64_t* tokens, const float* stats,
                              const float* entropy, void* dh, int dh_dtype, void* dw, int dw_dtype, void* work,
                              int64_t N, int64_t V, int64_t D, int prec, void* stream);
-int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int backward, int prec);
+int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int top_k, int backward, int prec);
 
 /* ---- token embedding (nn.Embedding, model.py:119, 149) ------------------------------------------- */
 

@@ -68,9 +68,9 @@ def test_head_logprobs_arguments():
     refused(bwd(P, P, P, 16, P, 16, P, P, P, P, 5, P, 0, P, 2, 8, 16, 0, None), "dtype")
     refused(bwd(P, P, P, 16, P, 16, P, None, P, P, 0, P, 0, P, 2, 8, 16, 0, None), "null")
     assert bwd(P, P, P, 16, P, 16, P, P, P, None, 0, None, 0, P, 2, 8, 16, 0, None) == L.ULM_OK  # nothing wanted
-    assert lib.ulm_lm_head_logprobs_work_bytes(-1, 8, 16, 0, 0) == -1
+    assert lib.ulm_lm_head_logprobs_work_bytes(-1, 8, 16, 0, 0, 0) == -1
     for n, v in ((1, 1), (7, 32000), (16384, 32000)):
-        assert 0 < lib.ulm_lm_head_logprobs_work_bytes(n, v, 64, 0, 0) <= lib.ulm_lm_head_logprobs_work_bytes(n, v, 64, 1, 0)
+        assert 0 < lib.ulm_lm_head_logprobs_work_bytes(n, v, 64, 0, 0, 0) < lib.ulm_lm_head_logprobs_work_bytes(n, v, 64, 32, 0, 0)
 
 
 def test_embedding_arguments():

@@ -81,7 +81,7 @@ SIGNATURES = {
     "ulm_lm_head_logprobs_fwd": (_I, [_P, _I64, _P, _I64] + [_P] * 7 + [_I64, _I64, _I64, _I, _I, _P]),
     "ulm_lm_head_logprobs_bwd": (_I, [_P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I, _P,
                                       _I64, _I64, _I64, _I, _P]),
-    "ulm_lm_head_logprobs_work_bytes": (_I64, [_I64, _I64, _I64, _I, _I]),
+    "ulm_lm_head_logprobs_work_bytes": (_I64, [_I64, _I64, _I64, _I, _I, _I]),
     "ulm_embedding_fwd": (_I, [_P, _P, _I, _I64, _P, _I, _I64, _I64, _I64, ctypes.c_float, _P]),
     "ulm_embedding_bwd": (_I, [_P, _P, _I, _P, _I, _P, _I64, _I64, _I64, ctypes.c_float, _P]),
     "ulm_embedding_bwd_work_bytes": (_I64, [_I64, _I64, _I64]),

@@ -866,7 +866,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int n1 = kb1 - kb0, nkb = n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int n1 = kb1 - kb0;
+        const int nkb = shape.parts ? 6 * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         for (int i = 0; i < nkb; ++i) {
           if (!wait_or_abort(&empty[stage], phase ^ 1u, abort_flag, DEVERR_GEMM_PRODUCER_WAIT)) {
@@ -877,12 +878,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           uint8_t* sb = sa + Cfg::A_BYTES;
           mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
           // k blocks of the first operand pair, then those of the second (shape.K2)
-          const bool s2 = i >= n1;
+          const int part = shape.parts ? i / n1 : 0;  // pair of operand parts (shape.parts)
+          const bool s2 = !shape.parts && i >= n1;
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
-          const int k0 = (s2 ? i - n1 : kb0 + i) * TC_BK;
-          const int oa = s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
+          const int oa = shape.parts ? GEMM_PART_A[part] : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = shape.parts ? GEMM_PART_B[part] : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d(ma, sa, &full[stage], k0, tc.mb * TC_BM, oa);
           } else {
@@ -961,7 +963,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? 6 * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1169,7 +1171,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int n1 = kb1 - kb0, nkb = n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int n1 = kb1 - kb0;
+        const int nkb = shape.parts ? 6 * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         const int row0 = tc.mb * BM + (int)rank * 128;
         const int col0 = tc.nb * BN + (int)rank * 128;
@@ -1183,12 +1186,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
           const uint32_t bar = leader_full + (uint32_t)(stage * sizeof(uint64_t));
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
           // k blocks of the first operand pair, then those of the second (shape.K2)
-          const bool s2 = i >= n1;
+          const int part = shape.parts ? i / n1 : 0;  // pair of operand parts (shape.parts)
+          const bool s2 = !shape.parts && i >= n1;
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
-          const int k0 = (s2 ? i - n1 : kb0 + i) * TC_BK;
-          const int oa = s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
+          const int oa = shape.parts ? GEMM_PART_A[part] : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = shape.parts ? GEMM_PART_B[part] : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d_pair(ma, sa, bar, k0, row0, oa);
           } else {
@@ -1264,7 +1268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? 6 * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1670,7 +1674,7 @@ int launch_tc(const Operand& A, const Operand& B, const Operand* A2, const Opera
               const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = TcConfig<BN>;
   CUtensorMap ta, tb, ta2, tb2, tout, taux;
-  const int ob = s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int ob = s.parts ? 3 : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
   int rc = make_tmap(&ta, A, ob, 64, A_MN ? 64 : TC_BM);
   if (rc) return rc;
   rc = make_tmap(&tb, B, ob, 64, B_MN ? 64 : BN);
@@ -1715,7 +1719,7 @@ int launch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Oper
                const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = Tc2Config;
   CUtensorMap ta, tb, ta2, tb2, tout, taux;
-  const int ob = s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int ob = s.parts ? 3 : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
   int rc = make_tmap(&ta, A, ob, 64, A_MN ? 64 : 128);
   if (rc) return rc;
   rc = make_tmap(&tb, B, ob, 64, B_MN ? 64 : 128);
@@ -1826,6 +1830,9 @@ int run_gemm2(const Operand& A, const Operand& B, const Operand* A2, const Opera
   ULM_REQUIRE(s.ksplit <= 1 || (s.causal == CAUSAL_NONE && s.ksplit == s.batches &&
                                  (int64_t)(s.ksplit - 1) * ksplit_chunk(s.K, s.ksplit) < s.K),
               "split K needs a non-causal product, batches == ksplit and no empty k range");
+  ULM_REQUIRE(!s.parts || (A.dtype == ULM_BF16 && s.batches == 1 && s.ksplit <= 1 && s.K2 == 0 && !s.carry &&
+                           s.causal == CAUSAL_NONE),
+              "operand parts need a plain product of bf16 parts");
   if (s.batches == 0 || s.M == 0 || s.N == 0) return ULM_OK;
   ULM_REQUIRE(s.K > 0, "empty contraction");
   if (A.dtype == ULM_BF16) {

@@ -6,7 +6,7 @@
 // over rows of logits x that exist already (ulm_token_logprobs_*), or that are x = h W^T
 // (ulm_lm_head_logprobs_*). Token -1 is padding: logp 0 and no a term. Any other token outside
 // [0, V) makes its row's logp and gradients NaN. All statistics are fp32.
-#include "gemm.cuh"
+#include "logprobs_mma.cu"
 
 namespace ulm {
 namespace {
@@ -14,8 +14,6 @@ namespace {
 constexpr int LP_THREADS = 256;
 constexpr int LP_GROUPS = 64;     // groups of threads whose maxima give the threshold of the top k
 constexpr int LP_CAP = 512;       // candidates of one row above the threshold
-constexpr int LP_MAX_TOP = 32;    // top_k of the entries
-constexpr float LOG2E = 1.4426950408889634f;
 
 // Running statistics of a set of logits: the maximum m (-inf for none), s = sum exp(x - m) and
 // u = sum exp(x - m) (x - m), taken about 0 while m is -inf (every term is then zero, or NaN).
@@ -262,23 +260,6 @@ __global__ void __launch_bounds__(LP_THREADS)
   }
 }
 
-// The backward's factors of one row: dx_v = ([v = t] a) - p_v (a + b (log p_v + H)).
-struct LpCoef {
-  float base, logs, c0, b, a;
-  int64_t t;
-};
-__device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* stats, const float* entropy,
-                                          const float* dlogprobs, const float* dentropy, int64_t r, int V) {
-  LpCoef c;
-  c.t = tokens[r];
-  c.base = stats[2 * r];
-  c.logs = stats[2 * r + 1];
-  c.a = c.t == -1 || !dlogprobs ? 0.f : dlogprobs[r];
-  if (c.t < -1 || c.t >= V) c.a = __uint_as_float(0x7FC00000u);
-  c.b = dentropy ? dentropy[r] : 0.f;
-  c.c0 = c.a + (c.b != 0.f ? c.b * entropy[r] : 0.f);
-  return c;
-}
 __device__ __forceinline__ float lp_dlogit(const LpCoef& c, float x, int64_t v) {
   const float logp = (x - c.base) - c.logs;
   const float p = fast_exp2(logp * LOG2E);
@@ -348,13 +329,43 @@ int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const floa
 
 bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
-inline int64_t lp_al(int64_t n) { return (n + 255) / 256 * 256; }
-inline int64_t lp_ld_logits(int64_t V) { return (V + 3) / 4 * 4; }
-// rows of logits held at once by the head entries
-int64_t lp_rows_at_once(int64_t N, int64_t V) {
-  int64_t r = (256ll << 20) / (lp_ld_logits(V) * 4) / 256 * 256;
-  r = r < 256 ? 256 : r;
-  return r < N ? r : N;
+int lp_sms() {
+  const int dev = current_device();
+  return dev >= 0 ? sm_count(dev) : 148;
+}
+
+// The work buffer of the head's entries.
+struct LpWork {
+  void *h_parts, *w_parts, *dx, *dx_parts;
+  float *part, *given;
+  float2* list;
+  int64_t bytes;
+};
+LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward, bool f32) {
+  char* p = static_cast<char*>(base);
+  auto take = [&](int64_t bytes) {
+    char* q = p;
+    p += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  LpWork w{};
+  const int64_t ldd = ulm_operand_ld(D), ldv = ulm_operand_ld(V);
+  if (f32) {
+    w.h_parts = take(3 * N * ldd * 2);
+    w.w_parts = take(3 * V * ldd * 2);
+  }
+  if (backward) {
+    w.dx = take(N * ldv * (f32 ? 4 : 2));
+    if (f32) w.dx_parts = take(3 * N * ldv * 2);
+  } else {
+    const LpShape s = lp_shape(N, V, D, f32, lp_sms());
+    const int64_t shares = N * lp_groups(s) * s.slots * 2;
+    w.part = reinterpret_cast<float*>(take(shares * 16));
+    w.list = reinterpret_cast<float2*>(take(shares * lp_list_k(k) * 8));
+    w.given = reinterpret_cast<float*>(take(N * 4));
+  }
+  w.bytes = p - static_cast<char*>(base);
+  return w;
 }
 
 int lp_head_check(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens, int64_t N,
@@ -365,16 +376,6 @@ int lp_head_check(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w
   ULM_REQUIRE(N == 0 || (h_op && w_op), "null pointer argument");
   ULM_REQUIRE(ld_h >= D && ld_w >= D, "row stride shorter than the row");
   return ULM_OK;
-}
-
-// logits of rows r0 .. r0 + n
-int lp_logits(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, int dt, float* logits, int64_t r0,
-              int64_t n, int64_t V, int64_t D, cudaStream_t st) {
-  const int64_t es = dt == ULM_F32 ? 4 : 2, ldl = lp_ld_logits(V);
-  Operand A{static_cast<const char*>(h_op) + r0 * ld_h * es, ld_h, n * ld_h, D, n, dt, false};
-  Operand Bw{w_op, ld_w, V * ld_w, D, V, dt, false};
-  GemmShape s{1, (int)n, (int)V, (int)D, CAUSAL_NONE};
-  return run_gemm(A, Bw, s, make_epilogue(EPI_STORE, ULM_F32, logits, ldl, n * ldl, nullptr), st);
 }
 
 }  // namespace
@@ -410,10 +411,10 @@ extern "C" int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentr
                                                                         dentropy, dlogits, ld_d, N, V, st);
 }
 
-extern "C" int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int backward, int prec) {
-  if (N < 0 || V < 0 || D < 0) return -1;
-  const int64_t logits = lp_al(lp_rows_at_once(N, V) * lp_ld_logits(V) * 4);
-  return logits + (backward ? lp_al(N * ulm_operand_ld(V) * (prec == ULM_PREC_FP32 ? 4 : 2)) : 0);
+extern "C" int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int top_k, int backward, int prec) {
+  if (N < 0 || V <= 0 || D <= 0 || top_k < 0 || top_k > LP_MAX_TOP) return -1;
+  if (N == 0) return 256;
+  return lp_work(nullptr, N, V, D, top_k, backward != 0, prec == ULM_PREC_FP32).bytes;
 }
 
 extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w,
@@ -425,18 +426,27 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
   if (N == 0) return ULM_OK;
   ULM_REQUIRE(logprobs && entropy && work, "null pointer argument");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int dt = prec == ULM_PREC_FP32 ? ULM_F32 : ULM_BF16;
-  float* logits = static_cast<float*>(work);
-  const int64_t step = lp_rows_at_once(N, V);
-  for (int64_t r0 = 0; r0 < N; r0 += step) {
-    const int64_t n = N - r0 < step ? N - r0 : step;
-    if (int rc = lp_logits(h_op, ld_h, w_op, ld_w, dt, logits, r0, n, V, D, st)) return rc;
-    if (int rc = lp_rows_fwd(logits, ULM_F32, lp_ld_logits(V), tokens + r0, logprobs + r0, entropy + r0,
-                             stats ? stats + 2 * r0 : nullptr, top_ids ? top_ids + r0 * top_k : nullptr,
-                             top_logprobs ? top_logprobs + r0 * top_k : nullptr, n, V, top_k, st))
-      return rc;
-  }
-  return ULM_OK;
+  const bool f32 = prec == ULM_PREC_FP32;
+  const LpShape s = lp_shape(N, V, D, f32, lp_sms());
+  const LpWork w = lp_work(work, N, V, D, top_k, false, f32);
+  ULM_REQUIRE(lp_groups(s) * s.slots * 2 <= LP_JOIN_MAX, "too many column groups");
+  CUtensorMap th, tw, to;
+  memset(&to, 0, sizeof(to));
+  if (int rc = lp_operand(&th, h_op, ld_h, N, D, f32, w.h_parts, st)) return rc;
+  if (int rc = lp_operand(&tw, w_op, ld_w, V, D, f32, w.w_parts, st)) return rc;
+  LpArgs a{};
+  a.tokens = tokens;
+  a.part = w.part;
+  a.list = w.list;
+  a.given = w.given;
+  a.groups = lp_groups(s);
+  const int K = lp_list_k(top_k);
+  const int rc = K == 0   ? lp_launch<LP_STATS, 0, false>(th, tw, to, s, a, st)
+                 : K == 8 ? lp_launch<LP_STATS, 8, false>(th, tw, to, s, a, st)
+                          : lp_launch<LP_STATS, 32, false>(th, tw, to, s, a, st);
+  if (rc) return rc;
+  return launch_pdl(lp_join_kernel, dim3((unsigned)cdiv(N, 4)), dim3(128), 0, st, s, a, K, logprobs, entropy, stats,
+                    top_ids, top_logprobs, top_k);
 }
 
 extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
@@ -452,34 +462,47 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
     if (dw) ULM_CUDA_TRY(cudaMemsetAsync(dw, 0, V * D * (dw_dtype == ULM_F32 ? 4 : 2), st));
     return ULM_OK;
   }
-  const int dt = prec == ULM_PREC_FP32 ? ULM_F32 : ULM_BF16;
-  const int64_t es = dt == ULM_F32 ? 4 : 2, ldv = ulm_operand_ld(V), step = lp_rows_at_once(N, V);
-  float* logits = static_cast<float*>(work);
-  char* dlogits = static_cast<char*>(work) + lp_al(step * lp_ld_logits(V) * 4);
-  for (int64_t r0 = 0; r0 < N; r0 += step) {
-    const int64_t n = N - r0 < step ? N - r0 : step;
-    if (int rc = lp_logits(h_op, ld_h, w_op, ld_w, dt, logits, r0, n, V, D, st)) return rc;
-    void* d = dlogits + r0 * ldv * es;
-    const float* da = dlogprobs ? dlogprobs + r0 : nullptr;
-    const float* db = dentropy ? dentropy + r0 : nullptr;
-    const int rc = dt == ULM_F32
-                       ? lp_rows_bwd_t<float, float>(logits, lp_ld_logits(V), tokens + r0, stats + 2 * r0, entropy + r0,
-                                                     da, db, d, ldv, n, V, st)
-                       : lp_rows_bwd_t<float, __nv_bfloat16>(logits, lp_ld_logits(V), tokens + r0, stats + 2 * r0,
-                                                             entropy + r0, da, db, d, ldv, n, V, st);
-    if (rc) return rc;
+  const bool f32 = prec == ULM_PREC_FP32;
+  const int64_t ldv = ulm_operand_ld(V), ldd = ulm_operand_ld(D);
+  const LpShape s = lp_shape(N, V, D, f32, lp_sms());
+  const LpWork w = lp_work(work, N, V, D, 0, true, f32);
+  CUtensorMap th, tw, to;
+  if (int rc = lp_operand(&th, h_op, ld_h, N, D, f32, w.h_parts, st)) return rc;
+  if (int rc = lp_operand(&tw, w_op, ld_w, V, D, f32, w.w_parts, st)) return rc;
+  ULM_REQUIRE(make_epi_tmap(&to, EPI_MODE_WARP, w.dx, f32 ? ULM_F32 : ULM_BF16, V, N, 1, ldv, N * ldv),
+              "no tensor map of the logits' gradient");
+  LpArgs a{};
+  a.tokens = tokens;
+  a.stats = stats;
+  a.entropy = entropy;
+  a.dlogprobs = dlogprobs;
+  a.dentropy = dentropy;
+  if (int rc = f32 ? lp_launch<LP_GRAD, 0, true>(th, tw, to, s, a, st) : lp_launch<LP_GRAD, 0, false>(th, tw, to, s, a, st))
+    return rc;
+  const void *dx = w.dx, *hh = h_op, *ww = w_op;
+  if (f32) {
+    const int64_t ctas = cdiv(N * ldv, 256 * 8);
+    if (int rc = launch_pdl(lp_split_kernel, dim3((unsigned)(ctas < 8192 ? ctas : 8192)), dim3(256), 0, st,
+                            static_cast<const float*>(w.dx), ldv, static_cast<__nv_bfloat16*>(w.dx_parts), ldv, N, V))
+      return rc;
+    dx = w.dx_parts;
+    hh = w.h_parts;
+    ww = w.w_parts;
+    ld_h = ld_w = ldd;
   }
+  // each product's operands are single matrices, or the three parts of one (its batches)
+  auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) {
+    GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
+    g.parts = f32 ? 6 : 0;
+    return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
+  };
   if (dh) {
     // dh = dx W: A = dx (rows, K-major over the vocabulary), B = W as [token][d] (MN-major)
-    Operand A{dlogits, ldv, N * ldv, V, N, dt, false};
-    Operand Bw{w_op, ld_w, V * ld_w, D, V, dt, true};
-    GemmShape s{1, (int)N, (int)D, (int)V, CAUSAL_NONE};
-    if (int rc = run_gemm(A, Bw, s, make_epilogue(EPI_STORE, dh_dtype, dh, D, N * D, nullptr), st)) return rc;
+    const Operand A{dx, ldv, N * ldv, V, N, ULM_BF16, false}, Bw{ww, ld_w, V * ld_w, D, V, ULM_BF16, true};
+    if (int rc = product(A, Bw, N, V, dh, dh_dtype)) return rc;
   }
   if (!dw) return ULM_OK;
   // dW = dx^T h: A = dx as [row][token] (MN-major), B = h as [row][d] (MN-major)
-  Operand A{dlogits, ldv, N * ldv, V, N, dt, true};
-  Operand Bh{h_op, ld_h, N * ld_h, D, N, dt, true};
-  GemmShape s{1, (int)V, (int)D, (int)N, CAUSAL_NONE};
-  return run_gemm(A, Bh, s, make_epilogue(EPI_STORE, dw_dtype, dw, D, V * D, nullptr), st);
+  const Operand A{dx, ldv, N * ldv, V, N, ULM_BF16, true}, Bh{hh, ld_h, N * ld_h, D, N, ULM_BF16, true};
+  return product(A, Bh, V, N, dw, dw_dtype);
 }

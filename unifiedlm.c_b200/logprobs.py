@@ -71,7 +71,7 @@ def lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision, stats=True):
     opt = _op_dtype(precision)
     h_op, ld_h = _operand(h.detach(), opt)
     w_op, ld_w = _operand(weight.detach(), opt)
-    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, precision), device=h.device, dtype=torch.uint8)
+    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, top_k, 0, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
         L.check(lib.ulm_lm_head_logprobs_fwd(h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(),
                                              lp.data_ptr(), ent.data_ptr(), _addr(st), ids.data_ptr(), tlp.data_ptr(),
@@ -89,7 +89,7 @@ def lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision
     opt = _op_dtype(precision)
     h_op, ld_h = _operand(h.detach(), opt)
     w_op, ld_w = _operand(weight.detach(), opt)
-    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 1, precision), device=h.device, dtype=torch.uint8)
+    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, 1, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
         L.check(lib.ulm_lm_head_logprobs_bwd(
             _addr(dlp), _addr(dent), h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(), stats.data_ptr(),
