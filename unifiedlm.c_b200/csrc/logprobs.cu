@@ -58,21 +58,6 @@ __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
   }
 }
 
-// Order of the alternatives as one integer: the value's bits made monotone (NaN above all, -0 = 0),
-// then the lower id.
-__device__ __forceinline__ uint64_t lp_key(float x, uint32_t id) {
-  uint32_t b = __float_as_uint(x + 0.f);
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (x != x) b = 0xFFFFFFFEu;
-  return ((uint64_t)b << 32) | (uint64_t)(0xFFFFFFFFu - id);
-}
-__device__ __forceinline__ float lp_key_value(uint64_t k) {
-  const uint32_t b = (uint32_t)(k >> 32);
-  if (b == 0xFFFFFFFEu) return __uint_as_float(0x7FC00000u);
-  return __uint_as_float((b & 0x80000000u) ? (b & 0x7FFFFFFFu) : ~b);
-}
-__device__ __forceinline__ uint32_t lp_key_id(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
-
 template <typename T>
 __device__ __forceinline__ float lp_load(const T* p);
 template <>
@@ -337,7 +322,7 @@ int lp_sms() {
 // The work buffer of the head's entries.
 struct LpWork {
   void *h_parts, *w_parts, *dx, *dx_parts;
-  float *part, *given;
+  float *part, *given, *dump;
   float2* list;
   int64_t bytes;
 };
@@ -361,7 +346,8 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     const LpShape s = lp_shape(N, V, D, f32, lp_sms());
     const int64_t shares = N * lp_groups(s) * s.slots * 2;
     w.part = reinterpret_cast<float*>(take(shares * 16));
-    w.list = reinterpret_cast<float2*>(take(shares * lp_list_k(k) * 8));
+    w.list = reinterpret_cast<float2*>(take(shares * k * 8));
+    w.dump = reinterpret_cast<float*>(take(shares * k * 128));
     w.given = reinterpret_cast<float*>(take(N * 4));
   }
   w.bytes = p - static_cast<char*>(base);
@@ -438,15 +424,17 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
   a.tokens = tokens;
   a.part = w.part;
   a.list = w.list;
+  a.dump = w.dump;
   a.given = w.given;
+  a.k = top_k;
   a.groups = lp_groups(s);
   const int K = lp_list_k(top_k);
   const int rc = K == 0   ? lp_launch<LP_STATS, 0, false>(th, tw, to, s, a, st)
                  : K == 8 ? lp_launch<LP_STATS, 8, false>(th, tw, to, s, a, st)
                           : lp_launch<LP_STATS, 32, false>(th, tw, to, s, a, st);
   if (rc) return rc;
-  return launch_pdl(lp_join_kernel, dim3((unsigned)cdiv(N, 4)), dim3(128), 0, st, s, a, K, logprobs, entropy, stats,
-                    top_ids, top_logprobs, top_k);
+  return launch_pdl(lp_join_kernel, dim3((unsigned)cdiv(N, LP_JOIN_WARPS)), dim3(32 * LP_JOIN_WARPS), 0, st, s, a,
+                    logprobs, entropy, stats, top_ids, top_logprobs);
 }
 
 extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,

@@ -3,17 +3,18 @@
 // tensor memory) with two epilogues.
 //
 // LP_STATS keeps, for each row, the running maximum, sum of exponentials and entropy sum of the softmax in
-// registers from tile to tile, and the best K logits in a sorted register list: an epilogue thread owns
-// half of a row's columns. A chunk of 32 logits costs its maximum and four instructions a logit; only
-// where the maximum beats the K-th best so far (about K ln(V / K) times a row) the warp looks for the
-// logits that do, reading them once more from tensor memory.
+// registers from tile to tile; an epilogue thread owns half of a row's columns, in chunks of 32 logits.
+// For the k best alternatives it keeps a sorted list of its k best chunks, by their maxima, and writes a
+// chunk that enters the list to the place of the one that leaves it (about k ln(chunks / k) times a row):
+// the k best logits lie in the k best chunks, so one comparison serves 32 logits.
 // LP_GRAD writes the logits' gradient ([v = t] a - p (a + b (log p + H))) in the operand type of the
 // products that follow.
 //
 // Each CTA pair takes one run of consecutive tiles, all of the same length to within one, in an order
 // that keeps a row block until its columns are done: h's tile and the rows' state stay, W streams from
 // L2. (One column group at a time where W does not fit there.) So all pairs end together whatever N and
-// V are, and a row block is cut into at most `slots` shares, which lp_join_kernel adds up.
+// V are, and a row block is cut into at most `slots` shares, which lp_join_kernel adds up,
+// looking through the k best chunks of each row.
 //
 // fp32 operands are given as three bf16 parts each (x = hi + mid + lo to the last bit, lp_split_kernel),
 // and the product runs over six pairs of parts, the small ones first: what is left out is below 2^-25 of
@@ -72,11 +73,14 @@ __device__ __forceinline__ LpTile lp_tile(const LpShape& s, int64_t t) {
 struct LpArgs {
   const int64_t* tokens;
   // LP_STATS: for share i = ((row * groups + g) * slots + slot) * 2 + half of a row: (max, sum, entropy sum)
-  // in part[4 i] (base 2: of 2^(x log2 e - max log2 e)), its best logits in list[i * K] as (value, id), and
-  // given[row], the token's logit
+  // in part[4 i] (base 2: of 2^(x log2 e - max log2 e)); its k best chunks in list[i * k + j], descending, as
+  // (maximum, chunk index * 32 + place), their logits in dump[(i * k + place) * 32]; and given[row], the
+  // token's logit
   float* part;
   float2* list;
+  float* dump;
   float* given;
+  int k;
   int groups;
   // LP_GRAD
   const float* stats;
@@ -84,15 +88,6 @@ struct LpArgs {
   const float* dlogprobs;
   const float* dentropy;
 };
-
-__device__ __forceinline__ void tmem_ld_32x1(uint32_t taddr, float& x) {
-  uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
-               : "=r"(r)
-               : "r"(taddr)
-               : "memory");
-  x = __uint_as_float(r);
-}
 
 // The backward's factors of one row: dx_v = ([v = t] a) - p_v (a + b (log p_v + H)).
 struct LpCoef {
@@ -112,40 +107,26 @@ __device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* st
   return c;
 }
 
-// The statistics of one thread's share of a row, over chunks of 32 logits.
+// The statistics of one thread's share of a row, over chunks of 32 logits; K is the most chunks that its
+// list can hold, the first K - k places are taken by +inf.
 template <int K>
 struct LpRun {
   float m, m2, s, u;  // maximum (at least -1e30), m log2 e, sum 2^(x log2 e - m2), sum 2^(.) (.)
   float v[K > 0 ? K : 1];
   int id[K > 0 ? K : 1];
 
-  __device__ __forceinline__ void reset(bool live) {
+  __device__ __forceinline__ void reset(bool live, int k) {
     m = -1e30f;
-    m2 = m * LOG2E;
+    m2 = __fmul_rn(m, LOG2E);
     s = u = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      v[j] = live ? -INFINITY : INFINITY;  // nothing beats the list of a row that is not there
-      id[j] = -1;
+      v[j] = live && j >= K - k ? -INFINITY : INFINITY;  // nothing enters the list of a row that is not there
+      id[j] = -32 + (j - (K - k));
     }
   }
-  __device__ __forceinline__ void insert(float x, int i) {
-#pragma unroll
-    for (int j = K - 1; j > 0; --j) {
-      const bool up = x > v[j - 1], here = x > v[j];
-      v[j] = up ? v[j - 1] : here ? x : v[j];
-      id[j] = up ? id[j - 1] : here ? i : id[j];
-    }
-    if (x > v[0]) {
-      v[0] = x;
-      id[0] = i;
-    }
-  }
-  // logits of columns col0 .. col0 + 31 (in tensor memory at taddr), V the first column past the last
-  __device__ __forceinline__ void add(const uint32_t (&r)[32], uint32_t taddr, int col0, int V) {
-    float x[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+  // logits x of columns col0 .. col0 + 31, V the first column past the last; dump: this share's chunks
+  __device__ __forceinline__ void add(float (&x)[32], int col0, int V, float* dump) {
     if (col0 + 32 > V) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) x[i] = col0 + i < V ? x[i] : -1e30f;
@@ -153,8 +134,27 @@ struct LpRun {
     float lm = fmaxf(x[0], x[1]);
 #pragma unroll
     for (int i = 2; i < 32; i += 2) lm = fmaxf(lm, fmaxf(x[i], x[i + 1]));
+    if (K > 0) {
+      if (lm > v[K - 1]) {
+        const int place = id[K - 1] & 31, mine = col0 | place;
+#pragma unroll
+        for (int j = K - 1; j > 0; --j) {
+          const bool up = lm > v[j - 1], here = lm > v[j];
+          v[j] = up ? v[j - 1] : here ? lm : v[j];
+          id[j] = up ? id[j - 1] : here ? mine : id[j];
+        }
+        if (lm > v[0]) {
+          v[0] = lm;
+          id[0] = mine;
+        }
+        float4* d = reinterpret_cast<float4*>(dump + place * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      }
+      __syncwarp();
+    }
     if (lm > m) {
-      const float n2 = lm * LOG2E, d = m2 - n2, f = fast_exp2(d);
+      const float n2 = __fmul_rn(lm, LOG2E), d = m2 - n2, f = fast_exp2(d);
       u = f > 0.f ? (u + s * d) * f : 0.f;
       s *= f;
       m = lm;
@@ -172,22 +172,6 @@ struct LpRun {
     }
     s += s0 + s1;
     u += u0 + u1;
-    if (K > 0) {
-      if (__any_sync(0xffffffffu, lm > v[K - 1])) {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) bits |= x[i] > v[K - 1] ? 1u << i : 0u;
-        bits = __reduce_or_sync(0xffffffffu, bits);
-        while (bits) {
-          const int i = __ffs(bits) - 1;
-          bits &= bits - 1;
-          float y;
-          tmem_ld_32x1(taddr + (uint32_t)i, y);
-          if (y > v[K - 1] && col0 + i < V) insert(y, col0 + i);
-          __syncwarp();
-        }
-      }
-    }
   }
 };
 
@@ -344,15 +328,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
     bool live = false;
     LpRun<K> run;
     LpCoef c;
-    if (MODE == LP_STATS) run.reset(false);
+    float* dump = nullptr;  // the chunks of this thread's share
+    int64_t share = 0;
+    if (MODE == LP_STATS) run.reset(false, 0);
     auto flush = [&]() {
       if (MODE != LP_STATS || at_rb < 0 || !live) return;
-      const int slot = pair - lp_pair_of(shape, lp_row_first(shape, at_g, at_rb));
-      const int64_t i = ((row * args.groups + at_g) * shape.slots + slot) * 2 + half;
-      *reinterpret_cast<float4*>(args.part + 4 * i) = make_float4(run.m, run.s, run.u, 0.f);
+      *reinterpret_cast<float4*>(args.part + 4 * share) = make_float4(run.m, run.s, run.u, 0.f);
       if (K > 0) {
 #pragma unroll
-        for (int q = 0; q < K; ++q) args.list[i * K + q] = make_float2(run.v[q], __int_as_float(run.id[q]));
+        for (int q = 0; q < K; ++q)
+          if (q >= K - args.k) args.list[share * args.k + q - (K - args.k)] = make_float2(run.v[q], __int_as_float(run.id[q]));
       }
     };
     for (int64_t t = t_first; t < t_end; ++t, ++j) {
@@ -364,7 +349,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         row = (int64_t)tile.rb * 256 + (int64_t)rank * 128 + quad * 32 + lane;
         live = row < shape.N;
         if (MODE == LP_STATS) {
-          run.reset(live);
+          const int slot = pair - lp_pair_of(shape, lp_row_first(shape, at_g, at_rb));
+          share = ((row * args.groups + at_g) * shape.slots + slot) * 2 + half;
+          dump = args.dump + share * args.k * 32;
+          run.reset(live, args.k);
           tok = live ? args.tokens[row] : -1;
         } else {
           c = live ? lp_coef(args.tokens, args.stats, args.entropy, args.dlogprobs, args.dentropy, row, shape.V)
@@ -380,32 +368,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
       const bool rows_here = __any_sync(0xffffffffu, live);
       const int chunks = rows_here ? min(4, (shape.V - col_base + 31) / 32) : 0;
       if (MODE == LP_STATS) {
+        // a list of 32 leaves no registers for the next chunk's load ahead
+        constexpr bool AHEAD = K <= 8;
         uint32_t ra[32], rb[32];
-        if (chunks > 0) tmem_ld_32x32_issue(taddr, ra);
-        auto one = [&](const uint32_t(&r)[32], int ch) {
+        if (AHEAD && chunks > 0) tmem_ld_32x32_issue(taddr, ra);
+        auto one = [&](uint32_t (&r)[32], uint32_t (&next)[32], int ch) {
           const int col0 = col_base + 32 * ch;
-          run.add(r, taddr + (uint32_t)(32 * ch), col0, shape.V);
+          if (!AHEAD) tmem_ld_32x32_issue(taddr + 32 * ch, r);
+          tmem_ld_32x32_wait(r);
+          if (AHEAD && ch + 1 < chunks) tmem_ld_32x32_issue(taddr + 32 * (ch + 1), next);
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+          run.add(x, col0, shape.V, dump);
           if (tok >= col0 && tok < col0 + 32 && tok < shape.V) {
             float g = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (col0 + i == (int)tok) g = __uint_as_float(r[i]);
+              if (col0 + i == (int)tok) g = x[i];
             args.given[row] = g;
           }
           __syncwarp();
         };
+        if (AHEAD) {
 #pragma unroll
-        for (int ch = 0; ch < 4; ch += 2) {
-          if (ch < chunks) {
-            tmem_ld_32x32_wait(ra);
-            if (ch + 1 < chunks) tmem_ld_32x32_issue(taddr + 32 * (ch + 1), rb);
-            one(ra, ch);
+          for (int ch = 0; ch < 4; ch += 2) {
+            if (ch < chunks) one(ra, rb, ch);
+            if (ch + 1 < chunks) one(rb, ra, ch + 1);
           }
-          if (ch + 1 < chunks) {
-            tmem_ld_32x32_wait(rb);
-            if (ch + 2 < chunks) tmem_ld_32x32_issue(taddr + 32 * (ch + 2), ra);
-            one(rb, ch + 1);
-          }
+        } else {
+#pragma unroll 1
+          for (int ch = 0; ch < chunks; ++ch) one(ra, rb, ch);
         }
       } else {
         constexpr int CW = F32 ? 32 : 64;  // columns of a staged chunk of 128 bytes a row
@@ -458,47 +451,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
   }
 }
 
-// One warp per row: its shares' statistics merged, its K-lists merged by k rounds of the best remaining
-// head (value descending, id ascending). Each lane keeps the heads of every 32nd list.
-__global__ void __launch_bounds__(128)
-    lp_join_kernel(const LpShape shape, const LpArgs args, int K, float* __restrict__ logprobs,
-                   float* __restrict__ entropy, float* __restrict__ stats, int64_t* __restrict__ top_ids,
-                   float* __restrict__ top_logprobs, int k) {
+// Order of the alternatives as one integer: the value's bits made monotone (NaN above all, -0 = 0),
+// then the lower id.
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t id) {
+  uint32_t b = __float_as_uint(x + 0.f);
+  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  if (x != x) b = 0xFFFFFFFEu;
+  return ((uint64_t)b << 32) | (uint64_t)(0xFFFFFFFFu - id);
+}
+__device__ __forceinline__ float lp_key_value(uint64_t k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  if (b == 0xFFFFFFFEu) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float((b & 0x80000000u) ? (b & 0x7FFFFFFFu) : ~b);
+}
+__device__ __forceinline__ uint32_t lp_key_id(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
+
+// A warp's rank of each key among n (all different) in shared memory: f(key index, rank)
+template <typename F>
+__device__ __forceinline__ void lp_rank(const uint64_t* key, int n, int lane, F&& f) {
+  for (int c = lane; c < n; c += 32) {
+    const uint64_t mine = key[c];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += key[j] > mine ? 1 : 0;
+    f(c, rank);
+  }
+}
+
+// One warp per row: its shares' statistics merged, then the k best logits of its chunks. Of the shares'
+// lists only those with the k best first chunks can hold one of the row's k best chunks, and of the row's
+// logits only those in its k best chunks (a chunk with k better ones ahead of it, in the order of maximum
+// and column, has k better logits ahead of all of its own). Each of the three choices is a rank among at
+// most 1024 keys, about k of them in the last two.
+constexpr int LP_JOIN_WARPS = 2;
+constexpr int LP_JOIN_MAX = 1024;  // shares of one row, and chunks or logits to choose from
+__global__ void __launch_bounds__(32 * LP_JOIN_WARPS)
+    lp_join_kernel(const LpShape shape, const LpArgs args, float* __restrict__ logprobs, float* __restrict__ entropy,
+                   float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+  __shared__ uint64_t keys[LP_JOIN_WARPS][LP_JOIN_MAX];
+  __shared__ int where[LP_JOIN_WARPS][LP_JOIN_MAX];
+  __shared__ int chosen[LP_JOIN_WARPS][LP_MAX_TOP];
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * LP_JOIN_WARPS + w;
   if (row >= shape.N) return;
-  const int rb = (int)(row / 256);
+  const int rb = (int)(row / 256), k = args.k;
   const int all = args.groups * shape.slots * 2;  // the row's possible shares
   // whether share i is there: its pair took tiles of this row block
-  auto there = [&](int i) {
-    const int g = i / (2 * shape.slots), slot = (i / 2) % shape.slots;
+  auto slots_of = [&](int g) {
     const int64_t a = lp_row_first(shape, g, rb), b = a + min(shape.group, shape.col_tiles - g * shape.group);
-    return lp_pair_of(shape, a) + slot <= lp_pair_of(shape, b - 1);
+    return lp_pair_of(shape, b - 1) - lp_pair_of(shape, a) + 1;
   };
-  uint32_t mine = 0;  // bit j: share lane + 32 j is there
-  for (int j = 0; 32 * j + lane < all; ++j) mine |= there(32 * j + lane) ? 1u << j : 0u;
+  const int slots0 = slots_of(0);
+  auto there = [&](int i) {
+    const int g = args.groups == 1 ? 0 : i / (2 * shape.slots);
+    return i < all && i / 2 - g * shape.slots < (g == 0 ? slots0 : slots_of(g));
+  };
   const float4* part = reinterpret_cast<const float4*>(args.part) + row * all;
-  float m = -1e30f;
-  for (int i = lane, j = 0; i < all; i += 32, ++j)
-    if ((mine >> j) & 1u) m = fmaxf(m, part[i].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float m2 = m * LOG2E;
-  float s = 0.f, u = 0.f;
-  for (int i = lane, j = 0; i < all; i += 32, ++j)
-    if ((mine >> j) & 1u) {
-      const float4 p = part[i];
-      const float d = p.x * LOG2E - m2, f = fast_exp2(d);
-      s = fmaf(p.y, f, s);
-      if (f > 0.f) u += (p.z + p.y * d) * f;
+  // sums are relative to m2 = fl(max log2 e), here as in the shares
+  float m = -1e30f, m2 = __fmul_rn(m, LOG2E), s = 0.f, u = 0.f;
+  for (int i = lane; i < all; i += 32) {
+    if (!there(i)) continue;
+    const float4 p = part[i];
+    const float p2 = __fmul_rn(p.x, LOG2E);
+    if (p.x > m) {
+      const float d = m2 - p2, f = fast_exp2(d);
+      u = f > 0.f ? (u + s * d) * f : 0.f;
+      s *= f;
+      m = p.x;
+      m2 = p2;
     }
+    const float d = p2 - m2, f = fast_exp2(d);
+    s = fmaf(p.y, f, s);
+    if (f > 0.f) u += (p.z + p.y * d) * f;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    u += __shfl_xor_sync(0xffffffffu, u, o);
+    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o),
+                ou = __shfl_xor_sync(0xffffffffu, u, o);
+    const float M = fmaxf(m, om), M2 = __fmul_rn(M, LOG2E);
+    const float da = __fmul_rn(m, LOG2E) - M2, fa = fast_exp2(da), db = __fmul_rn(om, LOG2E) - M2, fb = fast_exp2(db);
+    u = (fa > 0.f ? (u + s * da) * fa : 0.f) + (fb > 0.f ? (ou + os * db) * fb : 0.f);
+    s = s * fa + os * fb;
+    m = M;
+    m2 = M2;
   }
-  // logp = (x - m) - logs with log s + (m2 ln 2 - m), the second term the rounding of m2
+  // logp = (x - m) - logs: log s, and how far m2 ln 2 is from m
   const float logs = logf(s) + fmaf(LN2, m2, -m);
   if (lane == 0) {
     const int64_t t = args.tokens[row];
@@ -510,55 +548,82 @@ __global__ void __launch_bounds__(128)
     }
   }
   if (k == 0) return;
-  const float2* list = args.list + row * all * K;
-  uint32_t used[8];  // how many of each of its lists' entries a lane has given, 8 bits each
-#pragma unroll
-  for (int i = 0; i < 8; ++i) used[i] = 0;
-  for (int r = 0; r < k; ++r) {
-    float bv = -INFINITY;
-    int bid = 0x7fffffff, bl = -1;
-#pragma unroll
-    for (int w = 0; w < 8; ++w)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = lane + 32 * (4 * w + q);
-        if ((mine >> (4 * w + q)) & 1u) {
-          const int at = (used[w] >> (8 * q)) & 255;
-          if (at < K) {
-            const float2 e = list[(int64_t)i * K + at];
-            const int id = __float_as_int(e.y);
-            if (id >= 0 && (e.x > bv || (e.x == bv && id < bid))) {
-              bv = e.x;
-              bid = id;
-              bl = 4 * w + q;
-            }
-          }
-        }
-      }
-    float wv = bv;
-    int wid = bid;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, wv, o);
-      const int oid = __shfl_xor_sync(0xffffffffu, wid, o);
-      if (oid != 0x7fffffff && (wid == 0x7fffffff || ov > wv || (ov == wv && oid < wid))) {
-        wv = ov;
-        wid = oid;
-      }
+  const float2* list = args.list + row * all * k;
+  const float* dump = args.dump + row * all * k * 32;
+  uint64_t* key = keys[w];
+  int* at = where[w];
+  const uint32_t below = (1u << lane) - 1u;
+  int n = 0;  // entries collected
+  auto put = [&](bool yes, uint64_t kk, int ref) {
+    const uint32_t b = __ballot_sync(0xffffffffu, yes);
+    if (yes) {
+      key[n + __popc(b & below)] = kk;
+      at[n + __popc(b & below)] = ref;
     }
-    if (bl >= 0 && bid == wid) {
-#pragma unroll
-      for (int w = 0; w < 8; ++w)
-        if (bl / 4 == w) used[w] += 1u << (8 * (bl % 4));
+    n += __popc(b);
+  };
+  // the first chunks of the shares' lists
+  for (int i0 = 0; i0 < all; i0 += 32) {
+    const int i = i0 + lane;
+    const bool yes = there(i);
+    float2 e = make_float2(0.f, 0.f);
+    if (yes) e = list[(int64_t)i * k];
+    const int id = __float_as_int(e.y);
+    put(yes && id >= 0, lp_key(e.x, (uint32_t)(id >> 5)), i);
+  }
+  __syncwarp();
+  const int heads = n;
+  lp_rank(key, heads, lane, [&](int c, int rank) {
+    if (rank < k) chosen[w][rank] = at[c];
+  });
+  __syncwarp();
+  const int lists = min(heads, k);
+  // their chunks down to the k-th best first one
+  uint64_t floor_key = 0;
+  if (heads >= k) {
+    const float2 e = list[(int64_t)chosen[w][k - 1] * k];
+    floor_key = lp_key(e.x, (uint32_t)(__float_as_int(e.y) >> 5));
+  }
+  __syncwarp();
+  n = 0;
+  for (int l = 0; l < lists; ++l) {
+    const int i = chosen[w][l];
+    float2 e = make_float2(0.f, __int_as_float(-1));
+    if (lane < k) e = list[(int64_t)i * k + lane];
+    const int id = __float_as_int(e.y);
+    const uint64_t kk = lp_key(e.x, (uint32_t)(id >> 5));
+    put(id >= 0 && kk >= floor_key, kk, i * k + (id & 31));
+  }
+  __syncwarp();
+  const int chunks = n, best = min(chunks, k);
+  lp_rank(key, chunks, lane, [&](int c, int rank) {
+    if (rank < k) chosen[w][rank] = c;
+  });
+  __syncwarp();
+  // lane j keeps the j-th best chunk; the last one's maximum bounds the k-th best logit from below
+  const uint64_t ckey = lane < best ? key[chosen[w][lane]] : 0;
+  const int cat = lane < best ? at[chosen[w][lane]] : 0;
+  const float least = best == k ? lp_key_value(__shfl_sync(0xffffffffu, ckey, k - 1)) : -INFINITY;
+  __syncwarp();
+  n = 0;
+  for (int j = 0; j < best; ++j) {
+    const uint32_t id = lp_key_id(__shfl_sync(0xffffffffu, ckey, j)) * 32 + lane;
+    const float x = dump[(int64_t)__shfl_sync(0xffffffffu, cat, j) * 32 + lane];
+    put(id < (uint32_t)shape.V && x >= least, lp_key(x, id), 0);
+  }
+  __syncwarp();
+  lp_rank(key, n, lane, [&](int c, int rank) {
+    if (rank < k) {
+      top_ids[row * k + rank] = lp_key_id(key[c]);
+      top_logprobs[row * k + rank] = (lp_key_value(key[c]) - m) - logs;
     }
-    if (lane == 0) {
-      const bool none = wid == 0x7fffffff;  // only a row of NaN logits has fewer than k
-      top_ids[row * k + r] = none ? r : wid;
-      top_logprobs[row * k + r] = none ? __uint_as_float(0x7FC00000u) : (wv - m) - logs;
-    }
+  });
+  // only a row with NaN among its logits has fewer than k others
+  if (lane >= n && lane < k) {
+    top_ids[row * k + lane] = lane;
+    top_logprobs[row * k + lane] = __uint_as_float(0x7FC00000u);
   }
 }
-constexpr int LP_JOIN_MAX = 1024;  // shares of one row that lp_join_kernel can merge
 constexpr int LP_MAX_GROUPS = 128;
 
 // hi, mid and lo of fp32 rows (n, d), ld apart, as three bf16 matrices of row stride ld_o
