@@ -1830,7 +1830,7 @@ int run_gemm2(const Operand& A, const Operand& B, const Operand* A2, const Opera
   ULM_REQUIRE(s.ksplit <= 1 || (s.causal == CAUSAL_NONE && s.ksplit == s.batches &&
                                  (int64_t)(s.ksplit - 1) * ksplit_chunk(s.K, s.ksplit) < s.K),
               "split K needs a non-causal product, batches == ksplit and no empty k range");
-  ULM_REQUIRE(!s.parts || (A.dtype == ULM_BF16 && s.batches == 1 && s.ksplit <= 1 && s.K2 == 0 && !s.carry &&
+  ULM_REQUIRE(!s.parts || (A.dtype == ULM_BF16 && (s.batches == 1 || s.ksplit > 1) && s.K2 == 0 && !s.carry &&
                            s.causal == CAUSAL_NONE),
               "operand parts need a plain product of bf16 parts");
   if (s.batches == 0 || s.M == 0 || s.N == 0) return ULM_OK;

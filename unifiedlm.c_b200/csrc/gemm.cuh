@@ -58,7 +58,7 @@ struct GemmShape {
   // steps' token identity); 0 = each 16-deep k slice summed apart, then added (smaller rounding)
   int k_in_order = 0;
   // > 0: fp32 operands as three bf16 parts each (hi, mid, lo: batches 0, 1, 2 of A and B, one output
-  // batch); the k range is walked once for each of the six pairs GEMM_PART_A / GEMM_PART_B, the small
+  // batch, or one for each range of ksplit); the k range is walked once for each of the six pairs GEMM_PART_A / GEMM_PART_B, the small
   // products first. Left out are the products below 2^-25 of the whole one.
   int parts = 0;
 };
