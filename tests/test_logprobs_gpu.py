@@ -181,8 +181,13 @@ def test_rows_backward(dtype, N, V):
         za, zb = (g if g is not None else torch.zeros(N).cuda() for g in (ga, gb))
         want = plain_dx(logp, ent, t, za, zb)
         size = logp.exp() * (za.abs()[:, None] + zb.abs()[:, None] * (logp.abs() + ent[:, None]))
+        # the statistics are sums of 2^(x log2 e - fl(m log2 e)): the exponent's two roundings, of a number up
+        # to 2 |m|, leave log p and H an absolute error of 4 u (1 + |m|), also where both are zero (V = 1)
+        base = 4 * U * (1 + x.detach().double().abs().amax(-1, keepdim=True))
+        size = size + logp.exp() * zb.abs()[:, None] * base
         assert d.dtype == dtype
-        assert_close(d, want, size * (4 * rs + 8 * U * (1 + logp.abs())) + 2 * HALF[dtype] * want.abs() + 1e-37)
+        assert_close(d, want, size * (4 * rs + 8 * U * (1 + logp.abs())) + logp.exp() * zb.abs()[:, None] * base +
+                     2 * HALF[dtype] * want.abs() + 1e-37)
     assert L.device_error() == 0
 
 

@@ -9,39 +9,50 @@ the norm is the same in every run. A norm that is not finite makes the factor wh
 gives (0 or NaN), as torch's function does. The work runs in libulm_b200.so (ulm_clip_grads) on the
 current stream. No CPU path.
 """
-import ctypes
 import math
+from array import array
 
 import torch
 
 from . import _lib as L
 
 
+_CODE = {torch.float32: L.ULM_F32, torch.bfloat16: L.ULM_BF16}
+
+
+def _codes(ts):
+    try:
+        return array("i", [_CODE[t.dtype] for t in ts])
+    except KeyError as e:
+        raise L.UlmError(f"unsupported element type {e.args[0]}") from None
+
+
 def _run(grads, outs, max_norm):
-    dev = grads[0].device
+    at = grads[0].get_device()
+    if not all(g.is_cuda for g in grads):
+        raise RuntimeError("gradient clipping runs on CUDA tensors only (no CPU path)")
+    if any(g.get_device() != at for g in grads):
+        raise ValueError("gradients on several GPUs: one device expected")
+    if any(g.layout is not torch.strided for g in grads):
+        raise ValueError("sparse gradients are not supported")
     n = len(grads)
-    for g in grads:
-        if not g.is_cuda:
-            raise RuntimeError("gradient clipping runs on CUDA tensors only (no CPU path)")
-        if g.device != dev:
-            raise ValueError(f"gradients on {dev} and {g.device}: one device expected")
-        if g.layout != torch.strided:
-            raise ValueError("sparse gradients are not supported")
     src = [g if g.is_contiguous() else g.contiguous() for g in grads]
     dst = None
-    if outs is not None:
+    if outs is grads:
+        dst = src
+    elif outs is not None:
         dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
                for g, s, o in zip(grads, src, outs)]
-    vp, i64, i32 = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
+    lib, dev = L.lib(), grads[0].device
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    work = torch.empty(int(L.lib().ulm_clip_grads_work_bytes(n)), device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        L.check(L.lib().ulm_clip_grads(
-            vp(*[t.data_ptr() for t in src]), vp(*[t.data_ptr() for t in dst]) if dst else None,
-            i64(*[t.numel() for t in src]), i32(*[L.dtype_code(t.dtype) for t in src]),
-            i32(*[L.dtype_code(t.dtype) for t in dst]) if dst else None, n, max_norm, L.ptr(norm), L.ptr(work),
-            L.stream_of(norm)))
-    if dst:
+    work = torch.empty(lib.ulm_clip_grads_work_bytes(n), device=dev, dtype=torch.uint8)
+    ptrs, counts, codes = array("Q", [t.data_ptr() for t in src]), array("q", [t.numel() for t in src]), _codes(src)
+    optrs, ocodes = (ptrs, codes) if dst is src else (array("Q", [t.data_ptr() for t in dst]), _codes(dst)) if dst else (None, None)
+    addr = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
+    with L.on(dev):
+        L.check(lib.ulm_clip_grads(addr(ptrs), addr(optrs), addr(counts), addr(codes), addr(ocodes), n, max_norm,
+                                   norm.data_ptr(), work.data_ptr(), L.stream_of(norm)))
+    if dst is not None:
         for o, d in zip(outs, dst):
             if d is not o:
                 o.copy_(d)
@@ -69,7 +80,7 @@ def clip_grads(grads, max_norm, out=None):
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
-    for g, o in zip(grads, outs):
+    for g, o in zip(grads, outs) if outs is not grads else ():
         if o.shape != g.shape:
             raise ValueError(f"output {tuple(o.shape)} for a gradient {tuple(g.shape)}")
         if o.device != g.device:

@@ -2,7 +2,9 @@
 //   n = sqrt(sum over all tensors of g^2),   f = min(1, max_norm / (n + 1e-6)),   out = f g
 // One launch per table of tensors adds up the squares, a second one scales. Squares are added in
 // fp64 (they do not overflow, and the sum's order does not show in the fp32 norm); each CTA's share of
-// the elements is fixed, so the norm has the same bits in every run.
+// the elements is fixed, so the norm has the same bits in every run. Both are bound by HBM; the second
+// walks the chunks backwards, so that it finds what the first one read last in L2, and leaves out a tensor
+// that stays as it is (in place, factor 1).
 #include <algorithm>
 #include <vector>
 
@@ -12,9 +14,10 @@ namespace ulm {
 namespace {
 
 constexpr int CLIP_THREADS = 256;
-constexpr int CLIP_CTAS = 592;       // partial sums of one launch
+constexpr int CLIP_CTAS = 1184;      // partial sums of one launch: 8 CTAs an SM
 constexpr int CLIP_TABLE = 256;      // tensors of one launch
 constexpr int64_t CLIP_CHUNK = 8192; // elements of one piece of work
+constexpr int CLIP_UNROLL = 4;       // 16-byte pieces of a thread in flight
 
 struct ClipTable {
   const void* in[CLIP_TABLE];
@@ -37,10 +40,55 @@ __device__ __forceinline__ int clip_tensor(const ClipTable& t, int chunk) {
   return lo;
 }
 
-__device__ __forceinline__ float clip_load(const void* p, int dtype, int64_t i) {
-  return dtype == ULM_F32 ? static_cast<const float*>(p)[i]
-                          : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+template <typename T>
+__device__ __forceinline__ float clip_load(const T* p);
+template <>
+__device__ __forceinline__ float clip_load<float>(const float* p) {
+  return *p;
 }
+template <>
+__device__ __forceinline__ float clip_load<__nv_bfloat16>(const __nv_bfloat16* p) {
+  return __bfloat162float(*p);
+}
+__device__ __forceinline__ void clip_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void clip_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename T>
+struct ClipVec;
+template <>
+struct ClipVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[4]) {
+    x[0] = __uint_as_float(q.x);
+    x[1] = __uint_as_float(q.y);
+    x[2] = __uint_as_float(q.z);
+    x[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+template <>
+struct ClipVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
 
 __device__ __forceinline__ double clip_block_sum(double v, double* red) {
 #pragma unroll
@@ -53,20 +101,90 @@ __device__ __forceinline__ double clip_block_sum(double v, double* red) {
   return s;
 }
 
+// one(element) for the elements up to the first 16-byte boundary of p and after the last whole piece,
+// vec(piece index, piece) for the pieces between; n elements
+template <typename T, typename F1, typename FV>
+__device__ __forceinline__ void clip_walk(const T* p, int n, F1&& one, FV&& vec) {
+  int head = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  if (head > n) head = n;
+  const int nvec = (n - head) / ClipVec<T>::N, tail = head + nvec * ClipVec<T>::N + (int)threadIdx.x;
+  const uint4* body = reinterpret_cast<const uint4*>(p + head);
+  if ((int)threadIdx.x < head) one((int)threadIdx.x);
+  int i = threadIdx.x;
+  for (; i + (CLIP_UNROLL - 1) * CLIP_THREADS < nvec; i += CLIP_UNROLL * CLIP_THREADS) {
+    uint4 q[CLIP_UNROLL];
+#pragma unroll
+    for (int j = 0; j < CLIP_UNROLL; ++j) q[j] = body[i + j * CLIP_THREADS];
+#pragma unroll
+    for (int j = 0; j < CLIP_UNROLL; ++j) vec(i + j * CLIP_THREADS, q[j]);
+  }
+  for (; i < nvec; i += CLIP_THREADS) vec(i, body[i]);
+  if (tail < n) one(tail);
+}
+
+template <typename T>
+__device__ __forceinline__ double clip_square_chunk(const T* p, int n) {
+  double s = 0.0;
+  clip_walk(
+      p, n,
+      [&](int i) {
+        const double g = clip_load(p + i);
+        s += g * g;
+      },
+      [&](int, const uint4& q) {
+        float x[ClipVec<T>::N];
+        ClipVec<T>::unpack(q, x);
+#pragma unroll
+        for (int j = 0; j < ClipVec<T>::N; ++j) {
+          const double g = x[j];
+          s = fma(g, g, s);
+        }
+      });
+  return s;
+}
+
 __global__ void __launch_bounds__(CLIP_THREADS)
     grad_square_kernel(const __grid_constant__ ClipTable t, double* __restrict__ part) {
   __shared__ double red[CLIP_THREADS / 32];
+  pdl_enter();
   double s = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const int j = clip_tensor(t, c);
-    const int64_t i0 = (int64_t)(c - t.first[j]) * CLIP_CHUNK, i1 = min(t.n[j], i0 + CLIP_CHUNK);
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += CLIP_THREADS) {
-      const double g = clip_load(t.in[j], t.in_dtype[j], i);
-      s += g * g;
-    }
+    const int64_t i0 = (int64_t)(c - t.first[j]) * CLIP_CHUNK;
+    const int n = (int)min(CLIP_CHUNK, t.n[j] - i0);
+    s += t.in_dtype[j] == ULM_F32 ? clip_square_chunk(static_cast<const float*>(t.in[j]) + i0, n)
+                                  : clip_square_chunk(static_cast<const __nv_bfloat16*>(t.in[j]) + i0, n);
   }
   s = clip_block_sum(s, red);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+template <typename TI, typename TO>
+__device__ __forceinline__ void clip_scale_chunk(const TI* src, TO* dst, int n, float f) {
+  if (sizeof(TI) == sizeof(TO) && ((reinterpret_cast<uintptr_t>(src) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0) {
+    const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(TI)));
+    uint4* out = reinterpret_cast<uint4*>(dst + head);
+    clip_walk(
+        src, n, [&](int i) { clip_store(dst + i, clip_load(src + i) * f); },
+        [&](int i, const uint4& q) {
+          float x[ClipVec<TI>::N];
+          ClipVec<TI>::unpack(q, x);
+#pragma unroll
+          for (int j = 0; j < ClipVec<TI>::N; ++j) x[j] *= f;
+          out[i] = ClipVec<TI>::pack(x);
+        });
+    return;
+  }
+  // another type or another place in the 16 bytes: one element a thread, neighbours side by side
+  int i = threadIdx.x;
+  for (; i + 7 * CLIP_THREADS < n; i += 8 * CLIP_THREADS) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = clip_load(src + i + j * CLIP_THREADS);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) clip_store(dst + i + j * CLIP_THREADS, x[j] * f);
+  }
+  for (; i < n; i += CLIP_THREADS) clip_store(dst + i, clip_load(src + i) * f);
 }
 
 // the norm from all partial sums, and the clipped gradients
@@ -74,6 +192,7 @@ __global__ void __launch_bounds__(CLIP_THREADS)
     grad_clip_kernel(const __grid_constant__ ClipTable t, const double* __restrict__ part, int parts, float max_norm,
                      float* __restrict__ norm, int scale) {
   __shared__ double red[CLIP_THREADS / 32];
+  pdl_enter();
   double s = 0.0;
   for (int i = threadIdx.x; i < parts; i += CLIP_THREADS) s += part[i];
   s = clip_block_sum(s, red);
@@ -82,16 +201,24 @@ __global__ void __launch_bounds__(CLIP_THREADS)
   if (!scale) return;
   const float q = max_norm / (n + 1e-6f);
   const float f = q > 1.f ? 1.f : q;  // NaN stays
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const int j = clip_tensor(t, c);
-    const int64_t i0 = (int64_t)(c - t.first[j]) * CLIP_CHUNK, i1 = min(t.n[j], i0 + CLIP_CHUNK);
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += CLIP_THREADS) {
-      const float g = clip_load(t.in[j], t.in_dtype[j], i) * f;
-      if (t.out_dtype[j] == ULM_F32)
-        static_cast<float*>(t.out[j])[i] = g;
-      else
-        static_cast<__nv_bfloat16*>(t.out[j])[i] = __float2bfloat16_rn(g);
-    }
+    if (f == 1.f && t.in[j] == t.out[j]) continue;
+    const int64_t i0 = (int64_t)(c - t.first[j]) * CLIP_CHUNK;
+    const int m = (int)min(CLIP_CHUNK, t.n[j] - i0);
+    const bool i32 = t.in_dtype[j] == ULM_F32, o32 = t.out_dtype[j] == ULM_F32;
+    const float* fi = static_cast<const float*>(t.in[j]) + i0;
+    const __nv_bfloat16* bi = static_cast<const __nv_bfloat16*>(t.in[j]) + i0;
+    float* fo = static_cast<float*>(t.out[j]) + i0;
+    __nv_bfloat16* bo = static_cast<__nv_bfloat16*>(t.out[j]) + i0;
+    if (i32 && o32)
+      clip_scale_chunk(fi, fo, m, f);
+    else if (i32)
+      clip_scale_chunk(fi, bo, m, f);
+    else if (o32)
+      clip_scale_chunk(bi, fo, m, f);
+    else
+      clip_scale_chunk(bi, bo, m, f);
   }
 }
 
@@ -172,14 +299,14 @@ static int clip_grads_impl(const void* const* grads, void* const* outs, const in
   int parts = 0;
   for (const ClipTable& t : tables) {
     const int ctas = std::max(1, std::min(t.chunks, CLIP_CTAS));
-    grad_square_kernel<<<ctas, CLIP_THREADS, 0, st>>>(t, part + parts);
-    ULM_LAUNCH_CHECK("grad_square_kernel");
+    if (int rc = launch_pdl(grad_square_kernel, dim3(ctas), dim3(CLIP_THREADS), 0, st, t, part + parts)) return rc;
     parts += ctas;
   }
   for (const ClipTable& t : tables) {
     const int ctas = outs ? std::max(1, std::min(t.chunks, CLIP_CTAS)) : 1;
-    grad_clip_kernel<<<ctas, CLIP_THREADS, 0, st>>>(t, part, parts, max_norm, norm, outs ? 1 : 0);
-    ULM_LAUNCH_CHECK("grad_clip_kernel");
+    if (int rc = launch_pdl(grad_clip_kernel, dim3(ctas), dim3(CLIP_THREADS), 0, st, t, static_cast<const double*>(part),
+                            parts, max_norm, norm, outs ? 1 : 0))
+      return rc;
     if (!outs) break;
   }
   return ULM_OK;

@@ -13,49 +13,62 @@ namespace {
 
 constexpr int LP_THREADS = 256;
 constexpr int LP_GROUPS = 64;     // groups of threads whose maxima give the threshold of the top k
-constexpr int LP_CAP = 512;       // candidates of one row above the threshold
+constexpr int LP_CAP = 512;       // candidates of one CTA above the threshold
+constexpr int LP_MAX_SPLIT = 8;   // CTAs (one cluster) that share a row
 
-// Running statistics of a set of logits: the maximum m (-inf for none), s = sum exp(x - m) and
-// u = sum exp(x - m) (x - m), taken about 0 while m is -inf (every term is then zero, or NaN).
+// Running statistics of a set of logits in base 2: the maximum m (at least -1e30), m2 = fl(m log2 e),
+// s = sum 2^(x log2 e - m2) and u = sum 2^(.) (.).
 struct LpStat {
-  float m, s, u;
+  float m, m2, s, u;
+  __device__ __forceinline__ void raise(float to) {
+    const float n2 = __fmul_rn(to, LOG2E), d = m2 - n2, f = fast_exp2(d);
+    u = f > 0.f ? (u + s * d) * f : 0.f;
+    s *= f;
+    m = to;
+    m2 = n2;
+  }
 };
+constexpr float LP_LEAST = -1e30f;
 
-__device__ __forceinline__ LpStat lp_merge(const LpStat& a, const LpStat& b) {
+__device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b) {
   const float M = fmaxf(a.m, b.m);
-  auto part = [M](const LpStat& p, float& s, float& u) {
-    const float d = p.m == -INFINITY ? 0.f : p.m - M;
-    const float f = fast_exp2(d * LOG2E);
-    s = p.s * f;
-    u = f > 0.f ? (p.u + p.s * d) * f : 0.f;
-  };
-  float sa, ua, sb, ub;
-  part(a, sa, ua);
-  part(b, sb, ub);
-  return LpStat{M, sa + sb, ua + ub};
+  a.raise(M);
+  b.raise(M);
+  a.s += b.s;
+  a.u += b.u;
+  return a;
 }
 
-// NV more logits into a thread's statistics. fmaxf on the factor of u keeps exp(-inf) * -inf at 0.
+// NV more logits into a thread's statistics: the largest and the smallest first. Where a logit is below
+// -1e30 (-inf, or the type's lowest value, is a mask) its term is left out: 2^(.) is 0, but (.) may be
+// -inf.
 template <int NV>
 __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
-  float lm = x[0];
+  float hi = x[0], lo = x[0];
 #pragma unroll
-  for (int i = 1; i < NV; ++i) lm = fmaxf(lm, x[i]);
-  if (lm > st.m) {
-    const float d = st.m == -INFINITY ? 0.f : st.m - lm;
-    const float f = fast_exp2(d * LOG2E);
-    st.u = f > 0.f ? (st.u + st.s * d) * f : 0.f;
-    st.s *= f;
-    st.m = lm;
+  for (int i = 1; i < NV; ++i) {
+    hi = fmaxf(hi, x[i]);
+    lo = fminf(lo, x[i]);
   }
-  const float base = st.m == -INFINITY ? 0.f : st.m;
+  if (hi > st.m) st.raise(hi);
+  if (lo < LP_LEAST) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float d = fmaf(x[i], LOG2E, -st.m2), e = fast_exp2(d);
+      st.s += e;
+      st.u = e > 0.f ? fmaf(e, d, st.u) : st.u;
+    }
+    return;
+  }
+  float s1 = 0.f, u1 = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const float d = x[i] - base;
-    const float e = fast_exp2(d * LOG2E);
-    st.s += e;
-    st.u = fmaf(e, fmaxf(d, -1e4f), st.u);
+    const float d = fmaf(x[i], LOG2E, -st.m2), e = fast_exp2(d);
+    s1 += e;
+    u1 = fmaf(e, d, u1);
   }
+  st.s += s1;
+  st.u += u1;
 }
 
 template <typename T>
@@ -69,23 +82,26 @@ __device__ __forceinline__ float lp_load<__nv_bfloat16>(const __nv_bfloat16* p) 
   return __bfloat162float(*p);
 }
 
-// Logits of 16 bytes as floats.
+// Logits of 16 bytes as floats, and back.
 template <typename T>
 struct LpVec;
 template <>
 struct LpVec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[4]) {
+  static __device__ __forceinline__ void unpack(const uint4& q, float* x) {
     x[0] = __uint_as_float(q.x);
     x[1] = __uint_as_float(q.y);
     x[2] = __uint_as_float(q.z);
     x[3] = __uint_as_float(q.w);
   }
+  static __device__ __forceinline__ uint4 pack(const float* x) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
 };
 template <>
 struct LpVec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&x)[8]) {
+  static __device__ __forceinline__ void unpack(const uint4& q, float* x) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -93,30 +109,59 @@ struct LpVec<__nv_bfloat16> {
       x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
+  static __device__ __forceinline__ uint4 pack(const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 
-// Elements before the first 16-byte boundary of a row, at most n.
+// Elements before the first 16-byte boundary at p, at most n.
 template <typename T>
-__device__ __forceinline__ int lp_head(const T* row, int n) {
-  const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T));
+__device__ __forceinline__ int lp_head(const T* p, int n) {
+  const int h = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
   return h < n ? h : n;
 }
 
-// f(id, values) over the row's V logits, 16 bytes at a time from its first 16-byte boundary, and one
-// at a time at the two ends; thread t takes every LP_THREADS-th piece.
-template <typename T, typename F1, typename FV>
-__device__ __forceinline__ void lp_for_each(const T* row, int V, F1&& one, FV&& vec) {
-  constexpr int NV = LpVec<T>::N;
-  const int head = lp_head(row, V), nvec = (V - head) / NV, tail0 = head + nvec * NV;
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
-  if ((int)threadIdx.x < head) one((int)threadIdx.x, lp_load(row + threadIdx.x));
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nvec; i += LP_THREADS) {
+// f(id, values) over logits c0 .. c1 of a row, four 16-byte pieces at a time (16 fp32 or 32 bf16 logits, all
+// loaded before the first is used) from the first 16-byte boundary, one piece at a time where fewer are
+// left, and one logit at a time at the two ends.
+template <typename T, typename F>
+__device__ __forceinline__ void lp_for_each(const T* row, int c0, int c1, F&& f) {
+  constexpr int NV = LpVec<T>::N, U = 4;
+  const int n = c1 - c0, head = lp_head(row + c0, n), nvec = (n - head) / NV, tail0 = c0 + head + nvec * NV;
+  const uint4* body = reinterpret_cast<const uint4*>(row + c0 + head);
+  auto one = [&](int id) {
+    const float x[1] = {lp_load(row + id)};
+    const int ids[1] = {id};
+    f(ids, x);
+  };
+  if ((int)threadIdx.x < head) one(c0 + (int)threadIdx.x);
+  int i = threadIdx.x;
+  for (; i + (U - 1) * LP_THREADS < nvec; i += U * LP_THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) q[j] = body[i + j * LP_THREADS];
+    float x[U * NV];
+    int ids[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      LpVec<T>::unpack(q[j], x + j * NV);
+      ids[j] = c0 + head + (i + j * LP_THREADS) * NV;
+    }
+    f(ids, x);
+  }
+  for (; i < nvec; i += LP_THREADS) {
     float x[NV];
     LpVec<T>::unpack(body[i], x);
-    vec(head + i * NV, x);
+    const int ids[1] = {c0 + head + i * NV};
+    f(ids, x);
   }
-  if (tail0 + (int)threadIdx.x < V) one(tail0 + (int)threadIdx.x, lp_load(row + tail0 + threadIdx.x));
+  if (tail0 + (int)threadIdx.x < c1) one(tail0 + (int)threadIdx.x);
 }
 
 // The row's logp of its token from its statistics.
@@ -127,120 +172,190 @@ __device__ __forceinline__ float lp_given(const T* row, int64_t t, int V, float 
   return (lp_load(row + t) - base) - logs;
 }
 
-// One CTA per row.
+__device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t other = __shfl_xor_sync(0xffffffffu, v, o);
+    v = other > v ? other : v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < LP_THREADS / 32; ++w) v = red[w] > v ? red[w] : v;
+  return v;
+}
+
+// One cluster of `split` CTAs per row, each with an equal run of its columns. A CTA makes one pass over
+// its logits for the statistics and, for the alternatives, a second one out of L1 and L2 that compares with
+// a threshold: the k-th largest of 64 groups' maxima bounds the k-th best logit of the run from below, and
+// only about k logits reach it. The cluster's first CTA joins the runs. Bound by the pass over HBM for
+// many rows (4096 x 32000 bf16: 63 us, 4.1 TB/s), by latency for few: a row of 32000 split over 8 CTAs takes
+// 10 us, on one CTA 15.5 us.
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
     lp_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens,
                    float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ stats,
-                   int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int V, int k) {
+                   int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int V, int k, int split) {
   __shared__ LpStat part[LP_THREADS / 32];
+  __shared__ LpStat runs[LP_MAX_SPLIT];                    // of the cluster's CTAs (first CTA)
+  __shared__ uint64_t best[LP_MAX_SPLIT * LP_MAX_TOP];     // their alternatives, 0 for none (first CTA)
   __shared__ float gmax[LP_GROUPS];
   __shared__ float thr_s;
   __shared__ uint64_t cand[LP_CAP];
   __shared__ uint64_t red[LP_THREADS / 32];
   __shared__ int count;
+  pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
-  const int64_t r = blockIdx.x;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int64_t r = blockIdx.x / split;
   const T* row = x + r * ld;
-  LpStat st{-INFINITY, 0.f, 0.f};
-  lp_for_each(
-      row, V,
-      [&](int, float v) {
-        const float one[1] = {v};
-        lp_add(st, one);
-      },
-      [&](int, const auto& v) { lp_add(st, v); });
-  // the maxima of the groups of LP_THREADS / LP_GROUPS neighbouring threads
-  float g = st.m;
+  const int c0 = (int)((int64_t)V * rank / split), c1 = (int)((int64_t)V * (rank + 1) / split);
+  LpStat st{LP_LEAST, __fmul_rn(LP_LEAST, LOG2E), 0.f, 0.f};
+  lp_for_each(row, c0, c1, [&](const auto&, const auto& v) { lp_add(st, v); });
+  if (k > 0) {
+    // the maxima of the groups of LP_THREADS / LP_GROUPS neighbouring threads
+    float g = st.m;
 #pragma unroll
-  for (int o = LP_THREADS / LP_GROUPS / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  if (tid % (LP_THREADS / LP_GROUPS) == 0) gmax[tid / (LP_THREADS / LP_GROUPS)] = g;
+    for (int o = LP_THREADS / LP_GROUPS / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % (LP_THREADS / LP_GROUPS) == 0) gmax[tid / (LP_THREADS / LP_GROUPS)] = g;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const LpStat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                       __shfl_xor_sync(0xffffffffu, st.u, o)};
+    const LpStat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.m2, o),
+                       __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.u, o)};
     st = lp_merge(st, other);
   }
   if (lane == 0) part[wp] = st;
   if (tid == 0) count = 0;
   __syncthreads();
-  LpStat all = part[0];
+  if (tid == 0) {
+    LpStat all = part[0];
 #pragma unroll
-  for (int w = 1; w < LP_THREADS / 32; ++w) all = lp_merge(all, part[w]);
-  const float base = all.m == -INFINITY ? 0.f : all.m;
-  const float logs = logf(all.s);
+    for (int w = 1; w < LP_THREADS / 32; ++w) all = lp_merge(all, part[w]);
+    if (rank == 0) {
+      runs[0] = all;
+    } else {
+      const uint32_t to = mapa_shared(smem_u32(&runs[rank]), 0);
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(all.m), "f"(all.m2), "f"(all.s),
+                   "f"(all.u)
+                   : "memory");
+    }
+  }
+  if (k > 0) {
+    auto give = [&](int place, uint64_t key) {
+      const uint32_t to = mapa_shared(smem_u32(&best[rank * k + place]), 0);
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
+    };
+    if (tid < LP_GROUPS) {
+      int place = 0;
+      const float mine = gmax[tid];
+#pragma unroll 8
+      for (int j = 0; j < LP_GROUPS; ++j) place += (gmax[j] > mine || (gmax[j] == mine && j < tid)) ? 1 : 0;
+      if (place == k - 1) thr_s = mine;
+    }
+    __syncthreads();
+    // below -1e30 there is no threshold: fewer than k groups hold a logit that is not masked. Those
+    // above it are then taken, and masked ones in the order of their ids where they are fewer than k.
+    const float thr = thr_s;
+    const bool few = thr <= LP_LEAST;
+    lp_for_each(row, c0, c1, [&](const auto& ids, const auto& v) {
+      constexpr int NV = (int)(sizeof(v) / sizeof(float)), NI = (int)(sizeof(ids) / sizeof(int));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (few ? !(v[i] <= thr) : !(v[i] < thr)) {
+          const int at = atomicAdd(&count, 1);
+          if (at < LP_CAP) cand[at] = lp_key(v[i], (uint32_t)(ids[i / (NV / NI)] + i % (NV / NI)));
+        }
+      }
+    });
+    __syncthreads();
+    const int n = count;
+    if (n <= LP_CAP && (n >= k || !few)) {
+      // each candidate's place is the number of better ones
+      for (int c = tid; c < n; c += LP_THREADS) {
+        const uint64_t key = cand[c];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += cand[j] > key ? 1 : 0;
+        if (place < k) give(place, key);
+      }
+      if (n + tid < k) give(n + tid, 0);
+    } else {
+      // more equal logits than the list holds, or too few that are not masked: the best one after the
+      // last, k times
+      uint64_t last = ~0ull;
+      for (int j = 0; j < k; ++j) {
+        uint64_t top = 0;
+        lp_for_each(row, c0, c1, [&](const auto& ids, const auto& v) {
+          constexpr int NV = (int)(sizeof(v) / sizeof(float)), NI = (int)(sizeof(ids) / sizeof(int));
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const uint64_t key = lp_key(v[i], (uint32_t)(ids[i / (NV / NI)] + i % (NV / NI)));
+            if (key < last && key > top) top = key;
+          }
+        });
+        top = lp_block_max(top, red);
+        if (tid == 0) give(j, top);
+        last = top;
+      }
+    }
+  }
+  if (split > 1) cluster_sync_all(); else __syncthreads();
+  if (rank != 0) return;
+  LpStat all = runs[0];
+  for (int i = 1; i < split; ++i) all = lp_merge(all, runs[i]);
+  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e. A row below -1e30 throughout has its
+  // statistics about -1e30 empty: those of a maximum of its own are taken in a second look.
+  float base = all.m, logs = logf(all.s) + fmaf(-all.m, LOG2E, all.m2) * LN2, ent = logf(all.s) - LN2 * (all.u / all.s);
+  if (all.s == 0.f) {
+    float hi = -INFINITY;
+    for (int c = tid; c < V; c += LP_THREADS) hi = fmaxf(hi, lp_load(row + c));
+    const float top = lp_key_value(lp_block_max(lp_key(hi, 0), red));
+    double s = 0.0, u = 0.0;
+    for (int c = tid; c < V; c += LP_THREADS) {
+      const double d = (double)lp_load(row + c) - (double)top, e = exp(d);
+      s += e;
+      if (e > 0.0) u += e * d;
+    }
+    __shared__ double dred[2][LP_THREADS / 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    if (lane == 0) {
+      dred[0][wp] = s;
+      dred[1][wp] = u;
+    }
+    __syncthreads();
+    s = u = 0.0;
+#pragma unroll
+    for (int w = 0; w < LP_THREADS / 32; ++w) {
+      s += dred[0][w];
+      u += dred[1][w];
+    }
+    base = top;
+    logs = (float)log(s);  // NaN for a row of -inf alone
+    ent = (float)(log(s) - u / s);
+  }
   if (tid == 0) {
     logprobs[r] = lp_given(row, tokens[r], V, base, logs);
-    entropy[r] = logs - all.u / all.s;
+    entropy[r] = ent;
     if (stats) {
       stats[2 * r] = base;
       stats[2 * r + 1] = logs;
     }
   }
-  if (k == 0) return;
-  // The k-th largest group maximum bounds the k-th best logit from below: only logits not under it
-  // are candidates (about k of them, unless many are equal).
-  if (tid < LP_GROUPS) {
-    int rank = 0;
-    const float mine = gmax[tid];
-#pragma unroll 8
-    for (int j = 0; j < LP_GROUPS; ++j) rank += (gmax[j] > mine || (gmax[j] == mine && j < tid)) ? 1 : 0;
-    if (rank == k - 1) thr_s = mine;
-  }
-  __syncthreads();
-  const float thr = thr_s;
-  auto offer = [&](int id, float v) {
-    if (!(v < thr)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < LP_CAP) cand[at] = lp_key(v, (uint32_t)id);
-    }
-  };
-  lp_for_each(row, V, offer, [&](int id, const auto& v) {
-#pragma unroll
-    for (int i = 0; i < LpVec<T>::N; ++i) offer(id + i, v[i]);
-  });
-  __syncthreads();
-  const int n = count;
-  if (n <= LP_CAP) {
-    // each candidate's place is the number of better ones
-    for (int c = tid; c < n; c += LP_THREADS) {
-      const uint64_t key = cand[c];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
-      if (rank < k) {
-        top_ids[r * k + rank] = lp_key_id(key);
-        top_logprobs[r * k + rank] = (lp_key_value(key) - base) - logs;
-      }
-    }
-    return;
-  }
-  // many equal logits: the best one after the last, k times
-  uint64_t last = ~0ull;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
-    auto look = [&](int id, float v) {
-      const uint64_t key = lp_key(v, (uint32_t)id);
-      if (key < last && key > best) best = key;
-    };
-    lp_for_each(row, V, look, [&](int id, const auto& v) {
-#pragma unroll
-      for (int i = 0; i < LpVec<T>::N; ++i) look(id + i, v[i]);
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
-    __syncthreads();
-    if (lane == 0) red[wp] = best;
-    __syncthreads();
-    best = red[0];
-#pragma unroll
-    for (int w = 1; w < LP_THREADS / 32; ++w) best = red[w] > best ? red[w] : best;
-    last = best;
-    if (tid == 0) {
-      top_ids[r * k + j] = lp_key_id(best);
-      top_logprobs[r * k + j] = (lp_key_value(best) - base) - logs;
+  const int n = split * k;
+  for (int c = tid; c < n; c += LP_THREADS) {
+    const uint64_t key = best[c];
+    if (key == 0) continue;
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += best[j] > key ? 1 : 0;
+    if (place < k) {
+      top_ids[r * k + place] = lp_key_id(key);
+      top_logprobs[r * k + place] = (lp_key_value(key) - base) - logs;
     }
   }
 }
@@ -248,7 +363,7 @@ __global__ void __launch_bounds__(LP_THREADS)
 __device__ __forceinline__ float lp_dlogit(const LpCoef& c, float x, int64_t v) {
   const float logp = (x - c.base) - c.logs;
   const float p = fast_exp2(logp * LOG2E);
-  const float d = p == 0.f ? 0.f : p * (c.b != 0.f ? fmaf(c.b, logp, c.c0) : c.c0);
+  const float d = p == 0.f ? 0.f : p * fmaf(c.b, logp, c.c0);
   return (v == c.t ? c.a : 0.f) - d;
 }
 
@@ -263,40 +378,91 @@ __device__ __forceinline__ void lp_store<__nv_bfloat16>(__nv_bfloat16* p, float 
   *p = __float2bfloat16_rn(v);
 }
 
-template <typename T, typename TO>
+// Elementwise: CTA (row, run of LP_BWD_RUN columns). 16-byte pieces where both rows have the same place
+// in theirs, else one logit at a time. Bound by HBM (read and write).
+constexpr int LP_BWD_RUN = 16384;
+template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
     lp_rows_bwd_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens,
                        const float* __restrict__ stats, const float* __restrict__ entropy,
                        const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
-                       TO* __restrict__ dx, int64_t ld_dx, int V) {
+                       T* __restrict__ dx, int64_t ld_dx, int V) {
+  pdl_enter();
+  constexpr int NV = LpVec<T>::N, U = 4;
   const int64_t r = blockIdx.x;
   const LpCoef c = lp_coef(tokens, stats, entropy, dlogprobs, dentropy, r, V);
-  for (int v = threadIdx.x; v < V; v += LP_THREADS)
-    lp_store(dx + r * ld_dx + v, lp_dlogit(c, lp_load(x + r * ld + v), v));
+  const int c0 = blockIdx.y * LP_BWD_RUN, n = min(LP_BWD_RUN, V - c0), tid = threadIdx.x;
+  const T* src = x + r * ld + c0;
+  T* dst = dx + r * ld_dx + c0;
+  const bool same = ((reinterpret_cast<uintptr_t>(src) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
+  const int head = same ? lp_head(src, n) : n, nvec = (n - head) / NV;
+#pragma unroll 4
+  for (int i = tid; i < head; i += LP_THREADS) lp_store(dst + i, lp_dlogit(c, lp_load(src + i), c0 + i));
+  const uint4* sv = reinterpret_cast<const uint4*>(src + head);
+  uint4* dv = reinterpret_cast<uint4*>(dst + head);
+  auto piece = [&](const uint4& q, int i) {
+    float v[NV];
+    LpVec<T>::unpack(q, v);
+    const int id = c0 + head + i * NV;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = lp_dlogit(c, v[j], id + j);
+    dv[i] = LpVec<T>::pack(v);
+  };
+  int i = tid;
+  for (; i + (U - 1) * LP_THREADS < nvec; i += U * LP_THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) q[j] = sv[i + j * LP_THREADS];
+#pragma unroll
+    for (int j = 0; j < U; ++j) piece(q[j], i + j * LP_THREADS);
+  }
+  for (; i < nvec; i += LP_THREADS) piece(sv[i], i);
+  const int tail = head + nvec * NV + tid;
+  if (tail < n) lp_store(dst + tail, lp_dlogit(c, lp_load(src + tail), c0 + tail));
 }
 
+int lp_sms() {
+  const int dev = current_device();
+  return dev >= 0 ? sm_count(dev) : 148;
+}
+
+// A row is split over as many CTAs as fit on the GPU at once (4 of them an SM), each with 2048 logits at
+// least.
 int lp_rows_fwd(const void* x, int dtype, int64_t ld, const int64_t* tokens, float* logprobs, float* entropy,
                 float* stats, int64_t* top_ids, float* top_logprobs, int64_t N, int64_t V, int k, cudaStream_t st) {
+  int split = 1;
+  while (split < LP_MAX_SPLIT && N * split * 2 <= 4 * (int64_t)lp_sms() && V / (split * 2) >= 2048) split *= 2;
+  ULM_REQUIRE(N * split < (1ll << 31), "extent too large");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(N * split));
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   if (dtype == ULM_F32)
-    lp_rows_kernel<float><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const float*>(x), ld, tokens, logprobs, entropy,
-                                                              stats, top_ids, top_logprobs, (int)V, k);
+    ULM_CUDA_TRY(cudaLaunchKernelEx(&cfg, lp_rows_kernel<float>, static_cast<const float*>(x), ld, tokens, logprobs, entropy,
+                                    stats, top_ids, top_logprobs, (int)V, k, split));
   else
-    lp_rows_kernel<__nv_bfloat16><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ld, tokens,
-                                                                      logprobs, entropy, stats, top_ids, top_logprobs,
-                                                                      (int)V, k);
-  ULM_LAUNCH_CHECK("lp_rows_kernel");
+    ULM_CUDA_TRY(cudaLaunchKernelEx(&cfg, lp_rows_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(x), ld, tokens,
+                                    logprobs, entropy, stats, top_ids, top_logprobs, (int)V, k, split));
   return ULM_OK;
 }
 
-template <typename T, typename TO>
-int lp_rows_bwd_t(const void* x, int64_t ld, const int64_t* tokens, const float* stats, const float* entropy,
-                  const float* dlogprobs, const float* dentropy, void* dx, int64_t ld_dx, int64_t N, int64_t V,
-                  cudaStream_t st) {
-  lp_rows_bwd_kernel<T, TO><<<(unsigned)N, LP_THREADS, 0, st>>>(static_cast<const T*>(x), ld, tokens, stats, entropy,
-                                                                dlogprobs, dentropy, static_cast<TO*>(dx), ld_dx,
-                                                                (int)V);
-  ULM_LAUNCH_CHECK("lp_rows_bwd_kernel");
-  return ULM_OK;
+template <typename T>
+int lp_rows_bwd(const void* x, int64_t ld, const int64_t* tokens, const float* stats, const float* entropy,
+                const float* dlogprobs, const float* dentropy, void* dx, int64_t ld_dx, int64_t N, int64_t V,
+                cudaStream_t st) {
+  const int64_t runs = cdiv(V, LP_BWD_RUN);
+  ULM_REQUIRE(runs < 65536, "extent too large");
+  return launch_pdl(lp_rows_bwd_kernel<T>, dim3((unsigned)N, (unsigned)runs), dim3(LP_THREADS), 0, st,
+                    static_cast<const T*>(x), ld, tokens, stats, entropy, dlogprobs, dentropy, static_cast<T*>(dx), ld_dx,
+                    (int)V);
 }
 
 // out = the sum of `parts` arrays of n, in order
@@ -328,11 +494,6 @@ int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const floa
 }
 
 bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
-
-int lp_sms() {
-  const int dev = current_device();
-  return dev >= 0 ? sm_count(dev) : 148;
-}
 
 // The work buffer of the head's entries.
 struct LpWork {
@@ -406,10 +567,10 @@ extern "C" int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentr
   if (N == 0) return ULM_OK;
   ULM_REQUIRE(logits && stats && entropy && dlogits, "null pointer argument");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == ULM_F32 ? lp_rows_bwd_t<float, float>(logits, ld, tokens, stats, entropy, dlogprobs, dentropy,
-                                                        dlogits, ld_d, N, V, st)
-                          : lp_rows_bwd_t<__nv_bfloat16, __nv_bfloat16>(logits, ld, tokens, stats, entropy, dlogprobs,
-                                                                        dentropy, dlogits, ld_d, N, V, st);
+  return dtype == ULM_F32 ? lp_rows_bwd<float>(logits, ld, tokens, stats, entropy, dlogprobs, dentropy, dlogits, ld_d, N,
+                                               V, st)
+                          : lp_rows_bwd<__nv_bfloat16>(logits, ld, tokens, stats, entropy, dlogprobs, dentropy, dlogits,
+                                                       ld_d, N, V, st);
 }
 
 extern "C" int64_t ulm_lm_head_logprobs_work_bytes(int64_t N, int64_t V, int64_t D, int top_k, int backward, int prec) {

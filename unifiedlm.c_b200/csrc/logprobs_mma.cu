@@ -536,8 +536,8 @@ __global__ void __launch_bounds__(32 * LP_JOIN_WARPS)
     m = M;
     m2 = M2;
   }
-  // logp = (x - m) - logs: log s, and how far m2 ln 2 is from m
-  const float logs = logf(s) + fmaf(LN2, m2, -m);
+  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e
+  const float logs = logf(s) + fmaf(-m, LOG2E, m2) * LN2;
   if (lane == 0) {
     const int64_t t = args.tokens[row];
     logprobs[row] = t == -1 ? 0.f : t < 0 || t >= shape.V ? __uint_as_float(0x7FC00000u) : (args.given[row] - m) - logs;
