@@ -156,6 +156,17 @@ def eager(*ts):
     return True
 
 
+def first_order(name):
+    """Called in a backward: refuses the one that is to be differentiated again (create_graph)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative (create_graph)")
+
+
+def stream(device):
+    """The current stream of a device as a plain address (`stream_of` without its wrapper objects)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class _Here:
     def __enter__(self):
         return self

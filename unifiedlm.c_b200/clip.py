@@ -29,12 +29,13 @@ def _codes(ts):
 
 def _run(grads, outs, max_norm):
     at = grads[0].get_device()
-    if not all(g.is_cuda for g in grads):
-        raise RuntimeError("gradient clipping runs on CUDA tensors only (no CPU path)")
-    if any(g.get_device() != at for g in grads):
-        raise ValueError("gradients on several GPUs: one device expected")
-    if any(g.layout is not torch.strided for g in grads):
-        raise ValueError("sparse gradients are not supported")
+    for g in grads:
+        if g.get_device() != at or at < 0:
+            if not g.is_cuda:
+                raise RuntimeError("gradient clipping runs on CUDA tensors only (no CPU path)")
+            raise ValueError("gradients on several GPUs: one device expected")
+        if g.layout is not torch.strided:
+            raise ValueError("sparse gradients are not supported")
     n = len(grads)
     src = [g if g.is_contiguous() else g.contiguous() for g in grads]
     dst = None
@@ -51,7 +52,7 @@ def _run(grads, outs, max_norm):
     addr = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
     with L.on(dev):
         L.check(lib.ulm_clip_grads(addr(ptrs), addr(optrs), addr(counts), addr(codes), addr(ocodes), n, max_norm,
-                                   norm.data_ptr(), work.data_ptr(), L.stream_of(norm)))
+                                   norm.data_ptr(), work.data_ptr(), L.stream(norm.device)))
     if dst is not None:
         for o, d in zip(outs, dst):
             if d is not o:

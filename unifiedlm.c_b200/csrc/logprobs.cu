@@ -495,10 +495,12 @@ int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const floa
 
 bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
+constexpr int LP_MAX_K_SPLITS = 4;
+
 // The work buffer of the head's entries.
 struct LpWork {
   void *h_parts, *w_parts, *dx, *dx_parts;
-  float *part, *given, *dump;
+  float *part, *given, *dump, *sums;
   float2* list;
   int64_t bytes;
 };
@@ -517,7 +519,10 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
   }
   if (backward) {
     w.dx = take(N * ldv * (f32 ? 4 : 2));
-    if (f32) w.dx_parts = take(3 * N * ldv * 2);
+    if (f32)
+      w.dx_parts = take(3 * N * ldv * 2);
+    else  // partial sums of dh or dW, whichever is split
+      w.sums = reinterpret_cast<float*>(take(LP_MAX_K_SPLITS * std::max(N, V) * D * 4));
   } else {
     const LpShape s = lp_shape(N, V, D, f32, lp_sms());
     const int64_t shares = N * lp_groups(s) * s.slots * 2;
@@ -609,7 +614,10 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
                  : K == 8 ? lp_launch<LP_STATS, 8, false>(th, tw, to, s, a, st)
                           : lp_launch<LP_STATS, 32, false>(th, tw, to, s, a, st);
   if (rc) return rc;
-  return launch_pdl(lp_join_kernel, dim3((unsigned)cdiv(N, LP_JOIN_WARPS)), dim3(32 * LP_JOIN_WARPS), 0, st, s, a,
+  if (N <= 4 * (int64_t)lp_sms())
+    return launch_pdl(lp_join_kernel<128>, dim3((unsigned)N), dim3(128), 0, st, s, a, logprobs, entropy, stats, top_ids,
+                      top_logprobs);
+  return launch_pdl(lp_join_kernel<32>, dim3((unsigned)cdiv(N, LP_JOIN_ROWS)), dim3(32 * LP_JOIN_ROWS), 0, st, s, a,
                     logprobs, entropy, stats, top_ids, top_logprobs);
 }
 
@@ -659,16 +667,33 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   // products are taken over ranges of about 512, whose sums are added with rounding (at 1001 x 4099 x 288
   // the gradients' error falls from 8e-6 to below 2e-6). The ranges' sums take the place of the fp32
   // gradient of the logits, which its parts have replaced.
+  //
+  // A bf16 product whose 256 x 256 tiles fill the CTA pairs badly (8192 x 768: 96 tiles, two rounds of 74)
+  // is split over k too, where the rounds saved are worth writing and adding the partial sums.
+  const int pairs = lp_sms() / 2;
   auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) -> int {
     GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
-    if (!f32) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
-    g.parts = 6;
-    const int64_t room = N * ldv / (rows * D);
-    int splits = (int)std::min<int64_t>(room, cdiv(k, 512));
+    g.parts = f32 ? 6 : 0;
+    int splits = 1;
+    if (f32) {
+      splits = (int)std::min<int64_t>(N * ldv / (rows * D), cdiv(k, 512));
+    } else {
+      const int64_t tiles = cdiv(rows, 256) * cdiv(D, 256);
+      const double round_us = 2.0 * 256 * 256 * (double)k / 19e6;   // of all pairs, at 1400 TFLOP/s
+      const double part_us = (double)rows * (double)D * 8 / 6.5e6;  // a partial sum, written and read
+      double least = (double)cdiv(tiles, pairs) * round_us;
+      for (int c = 2; c <= LP_MAX_K_SPLITS && c * 4096 <= k; ++c) {
+        const double t = (double)cdiv(tiles * c, pairs) / c * round_us + c * part_us + 5.0;
+        if (t < least) {
+          least = t;
+          splits = c;
+        }
+      }
+    }
     if (splits > 1) splits = (int)cdiv(k, ksplit_chunk((int)k, splits));
     if (splits <= 1) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
     g.batches = g.ksplit = splits;
-    float* sums = static_cast<float*>(w.dx);
+    float* sums = f32 ? static_cast<float*>(w.dx) : w.sums;
     if (int rc = run_gemm(A, B, g, make_epilogue(EPI_STORE, ULM_F32, sums, D, rows * D, nullptr), st)) return rc;
     return launch_pdl(lp_add_kernel, dim3((unsigned)std::min<int64_t>(cdiv(rows * D, 256), 1 << 20)), dim3(256), 0, st,
                       static_cast<const float*>(sums), splits, rows * D, out, dtype);

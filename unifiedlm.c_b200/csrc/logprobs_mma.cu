@@ -466,35 +466,34 @@ __device__ __forceinline__ float lp_key_value(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t lp_key_id(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
 
-// A warp's rank of each key among n (all different) in shared memory: f(key index, rank)
-template <typename F>
-__device__ __forceinline__ void lp_rank(const uint64_t* key, int n, int lane, F&& f) {
-  for (int c = lane; c < n; c += 32) {
-    const uint64_t mine = key[c];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += key[j] > mine ? 1 : 0;
-    f(c, rank);
-  }
-}
-
-// One warp per row: its shares' statistics merged, then the k best logits of its chunks. Of the shares'
-// lists only those with the k best first chunks can hold one of the row's k best chunks, and of the row's
-// logits only those in its k best chunks (a chunk with k better ones ahead of it, in the order of maximum
-// and column, has k better logits ahead of all of its own). Each of the three choices is a rank among at
-// most 1024 keys, about k of them in the last two.
-constexpr int LP_JOIN_WARPS = 2;
+// TPR threads per row (a warp for many rows, 128 threads for few): the shares' statistics merged, then
+// the k best logits of the row's chunks. Of the shares' lists only those with the k best first chunks can
+// hold one of the row's k best chunks, and of the row's logits only those in its k best chunks (a chunk
+// with k better ones ahead of it, in the order of maximum and column, has k better logits ahead of all of
+// its own). Each of the three choices is a rank among at most 1024 keys, about k of them in the last two.
 constexpr int LP_JOIN_MAX = 1024;  // shares of one row, and chunks or logits to choose from
-__global__ void __launch_bounds__(32 * LP_JOIN_WARPS)
+constexpr int LP_JOIN_ROWS = 2;    // rows of a CTA when a warp has a row
+template <int TPR>
+__global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     lp_join_kernel(const LpShape shape, const LpArgs args, float* __restrict__ logprobs, float* __restrict__ entropy,
                    float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs) {
-  __shared__ uint64_t keys[LP_JOIN_WARPS][LP_JOIN_MAX];
-  __shared__ int where[LP_JOIN_WARPS][LP_JOIN_MAX];
-  __shared__ int chosen[LP_JOIN_WARPS][LP_MAX_TOP];
+  constexpr int ROWS = TPR == 32 ? LP_JOIN_ROWS : 1;
+  __shared__ uint64_t keys[ROWS][LP_JOIN_MAX];
+  __shared__ int where[ROWS][LP_JOIN_MAX];
+  __shared__ int chosen[ROWS][LP_MAX_TOP];
+  __shared__ int counts[ROWS][3];
+  __shared__ uint64_t bound[ROWS];
+  __shared__ float4 wred[TPR / 32];
   pdl_enter();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * LP_JOIN_WARPS + w;
+  const int tid = threadIdx.x % TPR, w = threadIdx.x / TPR;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + w;
   if (row >= shape.N) return;
+  auto sync = [] {
+    if (TPR == 32)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
   const int rb = (int)(row / 256), k = args.k;
   const int all = args.groups * shape.slots * 2;  // the row's possible shares
   // whether share i is there: its pair took tiles of this row block
@@ -507,38 +506,53 @@ __global__ void __launch_bounds__(32 * LP_JOIN_WARPS)
     const int g = args.groups == 1 ? 0 : i / (2 * shape.slots);
     return i < all && i / 2 - g * shape.slots < (g == 0 ? slots0 : slots_of(g));
   };
+  if (tid < 3) counts[w][tid] = 0;
   const float4* part = reinterpret_cast<const float4*>(args.part) + row * all;
+  const float2* list = args.list + row * all * k;
+  const float* dump = args.dump + row * all * k * 32;
   // sums are relative to m2 = fl(max log2 e), here as in the shares
   float m = -1e30f, m2 = __fmul_rn(m, LOG2E), s = 0.f, u = 0.f;
-  for (int i = lane; i < all; i += 32) {
+  auto merge = [&](float om, float os, float ou) {
+    const float M = fmaxf(m, om), M2 = __fmul_rn(M, LOG2E);
+    const float da = m2 - M2, fa = fast_exp2(da), db = __fmul_rn(om, LOG2E) - M2, fb = fast_exp2(db);
+    u = (fa > 0.f ? (u + s * da) * fa : 0.f) + (fb > 0.f ? (ou + os * db) * fb : 0.f);
+    s = s * fa + os * fb;
+    m = M;
+    m2 = M2;
+  };
+  sync();
+  for (int i = tid; i < all; i += TPR) {
     if (!there(i)) continue;
     const float4 p = part[i];
-    const float p2 = __fmul_rn(p.x, LOG2E);
-    if (p.x > m) {
-      const float d = m2 - p2, f = fast_exp2(d);
-      u = f > 0.f ? (u + s * d) * f : 0.f;
-      s *= f;
-      m = p.x;
-      m2 = p2;
+    if (k > 0) {  // the share's first chunk
+      const float2 e = list[(int64_t)i * k];
+      const int id = __float_as_int(e.y);
+      if (id >= 0) {
+        const int at = atomicAdd(&counts[w][0], 1);
+        keys[w][at] = lp_key(e.x, (uint32_t)(id >> 5));
+        where[w][at] = i;
+      }
     }
-    const float d = p2 - m2, f = fast_exp2(d);
-    s = fmaf(p.y, f, s);
-    if (f > 0.f) u += (p.z + p.y * d) * f;
+    merge(p.x, p.y, p.z);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o),
                 ou = __shfl_xor_sync(0xffffffffu, u, o);
-    const float M = fmaxf(m, om), M2 = __fmul_rn(M, LOG2E);
-    const float da = __fmul_rn(m, LOG2E) - M2, fa = fast_exp2(da), db = __fmul_rn(om, LOG2E) - M2, fb = fast_exp2(db);
-    u = (fa > 0.f ? (u + s * da) * fa : 0.f) + (fb > 0.f ? (ou + os * db) * fb : 0.f);
-    s = s * fa + os * fb;
-    m = M;
-    m2 = M2;
+    merge(om, os, ou);
+  }
+  if (TPR > 32) {
+    if ((tid & 31) == 0) wred[tid >> 5] = make_float4(m, s, u, 0.f);
+    sync();
+    m = -1e30f;
+    m2 = __fmul_rn(m, LOG2E);
+    s = u = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) merge(wred[i].x, wred[i].y, wred[i].z);
   }
   // logp = (x - m) - logs: log s, and how far m2 is from m log2 e
   const float logs = logf(s) + fmaf(-m, LOG2E, m2) * LN2;
-  if (lane == 0) {
+  if (tid == 0) {
     const int64_t t = args.tokens[row];
     logprobs[row] = t == -1 ? 0.f : t < 0 || t >= shape.V ? __uint_as_float(0x7FC00000u) : (args.given[row] - m) - logs;
     entropy[row] = logf(s) - LN2 * (u / s);
@@ -548,80 +562,91 @@ __global__ void __launch_bounds__(32 * LP_JOIN_WARPS)
     }
   }
   if (k == 0) return;
-  const float2* list = args.list + row * all * k;
-  const float* dump = args.dump + row * all * k * 32;
   uint64_t* key = keys[w];
   int* at = where[w];
-  const uint32_t below = (1u << lane) - 1u;
-  int n = 0;  // entries collected
-  auto put = [&](bool yes, uint64_t kk, int ref) {
-    const uint32_t b = __ballot_sync(0xffffffffu, yes);
-    if (yes) {
-      key[n + __popc(b & below)] = kk;
-      at[n + __popc(b & below)] = ref;
+  // f(key index, rank) for the keys among the k best of n (all different)
+  auto rank = [&](int n, auto&& f) {
+    for (int c = tid; c < n; c += TPR) {
+      const uint64_t mine = key[c];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) r += key[j] > mine ? 1 : 0;
+      if (r < k) f(c, r);
     }
-    n += __popc(b);
   };
-  // the first chunks of the shares' lists
-  for (int i0 = 0; i0 < all; i0 += 32) {
-    const int i = i0 + lane;
-    const bool yes = there(i);
-    float2 e = make_float2(0.f, 0.f);
-    if (yes) e = list[(int64_t)i * k];
-    const int id = __float_as_int(e.y);
-    put(yes && id >= 0, lp_key(e.x, (uint32_t)(id >> 5)), i);
-  }
-  __syncwarp();
-  const int heads = n;
-  lp_rank(key, heads, lane, [&](int c, int rank) {
-    if (rank < k) chosen[w][rank] = at[c];
+  sync();
+  const int heads = counts[w][0], lists = min(heads, k);
+  rank(heads, [&](int c, int r) {
+    chosen[w][r] = at[c];
+    if (r == k - 1) bound[w] = key[c];
   });
-  __syncwarp();
-  const int lists = min(heads, k);
-  // their chunks down to the k-th best first one
-  uint64_t floor_key = 0;
-  if (heads >= k) {
-    const float2 e = list[(int64_t)chosen[w][k - 1] * k];
-    floor_key = lp_key(e.x, (uint32_t)(__float_as_int(e.y) >> 5));
-  }
-  __syncwarp();
-  n = 0;
-  for (int l = 0; l < lists; ++l) {
-    const int i = chosen[w][l];
-    float2 e = make_float2(0.f, __int_as_float(-1));
-    if (lane < k) e = list[(int64_t)i * k + lane];
+  sync();
+  const uint64_t floor_key = heads >= k ? bound[w] : 0;  // the k-th best first chunk
+  // the chosen lists' chunks that are not under it
+#pragma unroll 4
+  for (int i = tid; i < lists * 32; i += TPR) {
+    const int l = chosen[w][i / 32], j = i % 32;
+    if (j >= k) continue;
+    const float2 e = list[(int64_t)l * k + j];
     const int id = __float_as_int(e.y);
     const uint64_t kk = lp_key(e.x, (uint32_t)(id >> 5));
-    put(id >= 0 && kk >= floor_key, kk, i * k + (id & 31));
-  }
-  __syncwarp();
-  const int chunks = n, best = min(chunks, k);
-  lp_rank(key, chunks, lane, [&](int c, int rank) {
-    if (rank < k) chosen[w][rank] = c;
-  });
-  __syncwarp();
-  // lane j keeps the j-th best chunk; the last one's maximum bounds the k-th best logit from below
-  const uint64_t ckey = lane < best ? key[chosen[w][lane]] : 0;
-  const int cat = lane < best ? at[chosen[w][lane]] : 0;
-  const float least = best == k ? lp_key_value(__shfl_sync(0xffffffffu, ckey, k - 1)) : -INFINITY;
-  __syncwarp();
-  n = 0;
-  for (int j = 0; j < best; ++j) {
-    const uint32_t id = lp_key_id(__shfl_sync(0xffffffffu, ckey, j)) * 32 + lane;
-    const float x = dump[(int64_t)__shfl_sync(0xffffffffu, cat, j) * 32 + lane];
-    put(id < (uint32_t)shape.V && x >= least, lp_key(x, id), 0);
-  }
-  __syncwarp();
-  lp_rank(key, n, lane, [&](int c, int rank) {
-    if (rank < k) {
-      top_ids[row * k + rank] = lp_key_id(key[c]);
-      top_logprobs[row * k + rank] = (lp_key_value(key[c]) - m) - logs;
+    if (id >= 0 && kk >= floor_key) {
+      const int to = atomicAdd(&counts[w][1], 1);
+      key[to] = kk;
+      at[to] = l * k + (id & 31);
     }
+  }
+  sync();
+  const int chunks = counts[w][1], best = min(chunks, k);
+  rank(chunks, [&](int c, int r) { chosen[w][r] = c; });
+  sync();
+  // thread j < best keeps the j-th best chunk; the last one's maximum bounds the k-th best logit from below
+  int mine_at = 0;
+  uint64_t mine_key = 0;
+  if (tid < best) {
+    mine_key = key[chosen[w][tid]];
+    mine_at = at[chosen[w][tid]];
+  }
+  sync();
+  if (tid < best) {
+    key[LP_JOIN_MAX - 32 + tid] = mine_key;
+    chosen[w][tid] = mine_at;
+  }
+  sync();
+  const float least = best == k ? lp_key_value(key[LP_JOIN_MAX - 32 + k - 1]) : -INFINITY;
+  constexpr int HOLD = 1024 / TPR;  // logits of a thread, read before the list of keys is overwritten
+  float x[HOLD];
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) {
+    const int i = tid + j * TPR;
+    x[j] = i < best * 32 ? dump[(int64_t)chosen[w][i / 32] * 32 + i % 32] : -INFINITY;
+  }
+  uint32_t first[HOLD];
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) {
+    const int i = tid + j * TPR;
+    first[j] = i < best * 32 ? lp_key_id(key[LP_JOIN_MAX - 32 + i / 32]) * 32 : 0;
+  }
+  sync();
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) {
+    const int i = tid + j * TPR;
+    const uint32_t id = first[j] + i % 32;
+    if (i < best * 32 && id < (uint32_t)shape.V && x[j] >= least) {
+      const int to = atomicAdd(&counts[w][2], 1);
+      key[to] = lp_key(x[j], id);
+    }
+  }
+  sync();
+  const int n = counts[w][2];
+  rank(n, [&](int c, int r) {
+    top_ids[row * k + r] = lp_key_id(key[c]);
+    top_logprobs[row * k + r] = (lp_key_value(key[c]) - m) - logs;
   });
   // only a row with NaN among its logits has fewer than k others
-  if (lane >= n && lane < k) {
-    top_ids[row * k + lane] = lane;
-    top_logprobs[row * k + lane] = __uint_as_float(0x7FC00000u);
+  if (tid >= n && tid < k) {
+    top_ids[row * k + tid] = tid;
+    top_logprobs[row * k + tid] = __uint_as_float(0x7FC00000u);
   }
 }
 constexpr int LP_MAX_GROUPS = 128;

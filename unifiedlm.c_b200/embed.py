@@ -20,7 +20,7 @@ def embedding_fwd_raw(tokens, weight, scale, out_bf16):
     with L.on(weight.device):
         L.check(L.lib().ulm_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), L.dtype_code(weight.dtype),
                                           weight.stride(0) if V > 1 else D, y.data_ptr(), L.dtype_code(dt), N, V, D,
-                                          scale, L.stream_of(weight)))
+                                          scale, L.stream(weight.device)))
     return y
 
 
@@ -33,7 +33,7 @@ def embedding_bwd_raw(tokens, dy, V, scale, dw_bf16):
     work = torch.empty(lib.ulm_embedding_bwd_work_bytes(N, V, D), device=dy.device, dtype=torch.uint8)
     with L.on(dy.device):
         L.check(lib.ulm_embedding_bwd(tokens.data_ptr(), dy.data_ptr(), L.dtype_code(dy.dtype), dw.data_ptr(),
-                                      L.dtype_code(dt), work.data_ptr(), N, V, D, scale, L.stream_of(dy)))
+                                      L.dtype_code(dt), work.data_ptr(), N, V, D, scale, L.stream(dy.device)))
     return dw
 
 
@@ -48,10 +48,10 @@ class _Embedding(torch.autograd.Function):
         return embedding_fwd_raw(tokens, weight, scale, out_bf16)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None
+        L.first_order("embedding")
         return None, embedding_bwd_raw(*ctx.saved_tensors, dy.contiguous(), *ctx.meta), None, None
 
 

@@ -75,7 +75,7 @@ def lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision, stats=True):
     with L.on(h.device):
         L.check(lib.ulm_lm_head_logprobs_fwd(h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(),
                                              lp.data_ptr(), ent.data_ptr(), _addr(st), ids.data_ptr(), tlp.data_ptr(),
-                                             work.data_ptr(), N, V, D, top_k, precision, L.stream_of(h)))
+                                             work.data_ptr(), N, V, D, top_k, precision, L.stream(h.device)))
     return out
 
 
@@ -94,7 +94,7 @@ def lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision
         L.check(lib.ulm_lm_head_logprobs_bwd(
             _addr(dlp), _addr(dent), h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(), stats.data_ptr(),
             ent.data_ptr(), _addr(dh), L.dtype_code(h.dtype), _addr(dw), L.dtype_code(weight.dtype), work.data_ptr(),
-            N, V, D, precision, L.stream_of(h)))
+            N, V, D, precision, L.stream(h.device)))
     return dh, dw
 
 
@@ -115,10 +115,10 @@ class _HeadLogprobs(torch.autograd.Function):
         return lp, ent, ids, tlp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dlp, dent, *unused):
         if dlp is None and dent is None:
             return None, None, None, None, None
+        L.first_order("lm_head_logprobs")
         dh, dw = lm_head_logprobs_bwd_raw(_grad_in(dlp), _grad_in(dent), *ctx.saved_tensors, ctx.precision,
                                           *ctx.needs_input_grad[:2])
         return dh, dw, None, None, None
@@ -186,7 +186,7 @@ def token_logprobs_fwd_raw(logits, tokens, top_k, stats=True):
     with L.on(logits.device):
         L.check(L.lib().ulm_token_logprobs_fwd(logits.data_ptr(), L.dtype_code(logits.dtype), _row_stride(logits),
                                                tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), _addr(st),
-                                               ids.data_ptr(), tlp.data_ptr(), N, V, top_k, L.stream_of(logits)))
+                                               ids.data_ptr(), tlp.data_ptr(), N, V, top_k, L.stream(logits.device)))
     return out
 
 
@@ -197,7 +197,7 @@ def token_logprobs_bwd_raw(dlp, dent, logits, tokens, stats, ent):
     with L.on(logits.device):
         L.check(L.lib().ulm_token_logprobs_bwd(_addr(dlp), _addr(dent), logits.data_ptr(), L.dtype_code(logits.dtype),
                                                _row_stride(logits), tokens.data_ptr(), stats.data_ptr(), ent.data_ptr(),
-                                               d.data_ptr(), V, N, V, L.stream_of(logits)))
+                                               d.data_ptr(), V, N, V, L.stream(logits.device)))
     return d
 
 
@@ -213,10 +213,10 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp, ent, ids, tlp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dlp, dent, *unused):
         if dlp is None and dent is None:
             return None, None, None
+        L.first_order("token_logprobs")
         return token_logprobs_bwd_raw(_grad_in(dlp), _grad_in(dent), *ctx.saved_tensors), None, None
 
 
