@@ -197,6 +197,14 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
                : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) shared -> global, tracked in
+// this thread's bulk async-group.
+__device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(smem_src)),
+               "r"(bytes)
+               : "memory");
+}
+
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // Wait until at most N of this thread's bulk groups still read their shared-memory source.
@@ -290,6 +298,12 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t local_saddr, uint32_t r
 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_saddr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_saddr) : "memory");
+}
+
+// The same without release: where the barrier hands over what the thread has finished reading (tensor
+// memory), and no store of its own, which a release would wait for.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_saddr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_saddr) : "memory");
 }
 
 // Split cluster barrier: every thread arrives (release) early and waits (acquire) later.

@@ -465,18 +465,40 @@ int lp_rows_bwd(const void* x, int64_t ld, const int64_t* tokens, const float* s
                     (int)V);
 }
 
-// out = the sum of `parts` arrays of n, in order
+// out = the sum of `parts` arrays of n, in order; four values a thread where all starts allow it
 __global__ void __launch_bounds__(256)
     lp_add_kernel(const float* __restrict__ part, int parts, int64_t n, void* __restrict__ out, int dtype) {
   pdl_enter();
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  auto store = [&](int64_t i, float v) {
+    if (dtype == ULM_F32)
+      static_cast<float*>(out)[i] = v;
+    else
+      static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  };
+  if (n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    for (int64_t i = i0; i < n / 4; i += step) {
+      float4 s = reinterpret_cast<const float4*>(part)[i];
+#pragma unroll 4
+      for (int p = 1; p < parts; ++p) {
+        const float4 v = reinterpret_cast<const float4*>(part + p * n)[i];
+        s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      }
+      if (dtype == ULM_F32) {
+        reinterpret_cast<float4*>(out)[i] = s;
+      } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(s.x, s.y), b = __floats2bfloat162_rn(s.z, s.w);
+        reinterpret_cast<uint2*>(out)[i] =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
+    }
+    return;
+  }
+  for (int64_t i = i0; i < n; i += step) {
     float s = 0.f;
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) s += part[p * n + i];
-    if (dtype == ULM_F32)
-      static_cast<float*>(out)[i] = s;
-    else
-      static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(s);
+    store(i, s);
   }
 }
 
@@ -614,11 +636,12 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
                  : K == 8 ? lp_launch<LP_STATS, 8, false>(th, tw, to, s, a, st)
                           : lp_launch<LP_STATS, 32, false>(th, tw, to, s, a, st);
   if (rc) return rc;
+  const int room = top_k > 0 ? lp_join_room(lp_groups(s) * s.slots * 2, top_k) : 0;
   if (N <= 4 * (int64_t)lp_sms())
-    return launch_pdl(lp_join_kernel<128>, dim3((unsigned)N), dim3(128), 0, st, s, a, logprobs, entropy, stats, top_ids,
-                      top_logprobs);
-  return launch_pdl(lp_join_kernel<32>, dim3((unsigned)cdiv(N, LP_JOIN_ROWS)), dim3(32 * LP_JOIN_ROWS), 0, st, s, a,
-                    logprobs, entropy, stats, top_ids, top_logprobs);
+    return launch_pdl(lp_join_kernel<128>, dim3((unsigned)N), dim3(128), (size_t)room * 12, st, s, a, logprobs, entropy,
+                      stats, top_ids, top_logprobs, room);
+  return launch_pdl(lp_join_kernel<32>, dim3((unsigned)cdiv(N, LP_JOIN_ROWS)), dim3(32 * LP_JOIN_ROWS),
+                    (size_t)room * 12 * LP_JOIN_ROWS, st, s, a, logprobs, entropy, stats, top_ids, top_logprobs, room);
 }
 
 extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
@@ -695,7 +718,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
     g.batches = g.ksplit = splits;
     float* sums = f32 ? static_cast<float*>(w.dx) : w.sums;
     if (int rc = run_gemm(A, B, g, make_epilogue(EPI_STORE, ULM_F32, sums, D, rows * D, nullptr), st)) return rc;
-    return launch_pdl(lp_add_kernel, dim3((unsigned)std::min<int64_t>(cdiv(rows * D, 256), 1 << 20)), dim3(256), 0, st,
+    return launch_pdl(lp_add_kernel, dim3((unsigned)std::min<int64_t>(cdiv(rows * D, 1024), 1 << 20)), dim3(256), 0, st,
                       static_cast<const float*>(sums), splits, rows * D, out, dtype);
   };
   if (dh) {

@@ -36,6 +36,8 @@ constexpr int LPM_SLOTS = 2;  // 4 KB staging tiles of an epilogue warp (LP_GRAD
 constexpr uint32_t LPM_HALF_BYTES = 128 * 64 * 2;  // a CTA's 128 rows of one operand, 64 k values
 constexpr uint32_t LPM_STAGE_BYTES = 2 * LPM_HALF_BYTES;
 constexpr uint32_t LPM_SMEM = LPM_STAGES * LPM_STAGE_BYTES + EPI_WARPS * LPM_SLOTS * 4096u + 1024 + 512;
+constexpr int LPM_ROW = 144;  // bytes between the threads' chunks of LP_STATS: no two lanes of a quarter meet
+static_assert(32 * LPM_ROW <= LPM_SLOTS * 4096, "a warp's chunks fit its staging tiles");
 static_assert(LPM_SMEM <= 232448, "shared memory of one CTA");
 
 // The shape of a launch; total tiles are dealt to `pairs` CTA pairs, pair p the run [first(p), first(p + 1)).
@@ -125,8 +127,10 @@ struct LpRun {
       id[j] = -32 + (j - (K - k));
     }
   }
-  // logits x of columns col0 .. col0 + 31, V the first column past the last; dump: this share's chunks
-  __device__ __forceinline__ void add(float (&x)[32], int col0, int V, float* dump) {
+  // logits x of columns col0 .. col0 + 31, V the first column past the last; dump: this share's chunks in
+  // global memory, stage: this thread's 128 bytes of shared memory. A chunk that enters the list leaves by a
+  // bulk copy of its own: 32 rows' chunks lie far apart, and plain stores of them kept the warp waiting.
+  __device__ __forceinline__ void add(float (&x)[32], int col0, int V, float* dump, uint8_t* stage) {
     if (col0 + 32 > V) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) x[i] = col0 + i < V ? x[i] : -1e30f;
@@ -147,9 +151,13 @@ struct LpRun {
           v[0] = lm;
           id[0] = mine;
         }
-        float4* d = reinterpret_cast<float4*>(dump + place * 32);
+        bulk_wait_group_read<0>();  // the chunk before has left the stage
+        float4* d = reinterpret_cast<float4*>(stage);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        fence_proxy_async_smem();
+        bulk_store(dump + place * 32, stage, 128);
+        bulk_commit_group();
       }
       __syncwarp();
     }
@@ -380,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
           float x[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
-          run.add(x, col0, shape.V, dump);
+          run.add(x, col0, shape.V, dump, slots + lane * LPM_ROW);
           if (tok >= col0 && tok < col0 + 32 && tok < shape.V) {
             float g = 0.f;
 #pragma unroll
@@ -437,10 +445,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(leader_tempty + (uint32_t)(acc * sizeof(uint64_t)));
+      if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty + (uint32_t)(acc * sizeof(uint64_t)));
     }
     flush();
-    if (MODE == LP_GRAD && lane == 0) bulk_wait_group<0>();
+    bulk_wait_group<0>();
   }
 
   tc_fence_before();
@@ -476,11 +484,12 @@ constexpr int LP_JOIN_ROWS = 2;    // rows of a CTA when a warp has a row
 template <int TPR>
 __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     lp_join_kernel(const LpShape shape, const LpArgs args, float* __restrict__ logprobs, float* __restrict__ entropy,
-                   float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+                   float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs,
+                   int room) {
   constexpr int ROWS = TPR == 32 ? LP_JOIN_ROWS : 1;
-  __shared__ uint64_t keys[ROWS][LP_JOIN_MAX];
-  __shared__ int where[ROWS][LP_JOIN_MAX];
+  extern __shared__ uint64_t join_smem[];  // of each row: `room` keys, and as many places
   __shared__ int chosen[ROWS][LP_MAX_TOP];
+  __shared__ uint64_t best_key[ROWS][LP_MAX_TOP];
   __shared__ int counts[ROWS][3];
   __shared__ uint64_t bound[ROWS];
   __shared__ float4 wred[TPR / 32];
@@ -488,6 +497,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
   const int tid = threadIdx.x % TPR, w = threadIdx.x / TPR;
   const int64_t row = (int64_t)blockIdx.x * ROWS + w;
   if (row >= shape.N) return;
+  uint64_t* key = join_smem + w * room;
+  int* at = reinterpret_cast<int*>(join_smem + ROWS * room) + w * room;
   auto sync = [] {
     if (TPR == 32)
       __syncwarp();
@@ -528,9 +539,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
       const float2 e = list[(int64_t)i * k];
       const int id = __float_as_int(e.y);
       if (id >= 0) {
-        const int at = atomicAdd(&counts[w][0], 1);
-        keys[w][at] = lp_key(e.x, (uint32_t)(id >> 5));
-        where[w][at] = i;
+        const int to = atomicAdd(&counts[w][0], 1);
+        key[to] = lp_key(e.x, (uint32_t)(id >> 5));
+        at[to] = i;
       }
     }
     merge(p.x, p.y, p.z);
@@ -562,8 +573,6 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     }
   }
   if (k == 0) return;
-  uint64_t* key = keys[w];
-  int* at = where[w];
   // f(key index, rank) for the keys among the k best of n (all different)
   auto rank = [&](int n, auto&& f) {
     for (int c = tid; c < n; c += TPR) {
@@ -600,42 +609,21 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
   const int chunks = counts[w][1], best = min(chunks, k);
   rank(chunks, [&](int c, int r) { chosen[w][r] = c; });
   sync();
-  // thread j < best keeps the j-th best chunk; the last one's maximum bounds the k-th best logit from below
+  // the best chunks; the last one's maximum bounds the k-th best logit from below
   int mine_at = 0;
-  uint64_t mine_key = 0;
   if (tid < best) {
-    mine_key = key[chosen[w][tid]];
+    best_key[w][tid] = key[chosen[w][tid]];
     mine_at = at[chosen[w][tid]];
   }
   sync();
-  if (tid < best) {
-    key[LP_JOIN_MAX - 32 + tid] = mine_key;
-    chosen[w][tid] = mine_at;
-  }
+  if (tid < best) chosen[w][tid] = mine_at;
   sync();
-  const float least = best == k ? lp_key_value(key[LP_JOIN_MAX - 32 + k - 1]) : -INFINITY;
-  constexpr int HOLD = 1024 / TPR;  // logits of a thread, read before the list of keys is overwritten
-  float x[HOLD];
-#pragma unroll
-  for (int j = 0; j < HOLD; ++j) {
-    const int i = tid + j * TPR;
-    x[j] = i < best * 32 ? dump[(int64_t)chosen[w][i / 32] * 32 + i % 32] : -INFINITY;
-  }
-  uint32_t first[HOLD];
-#pragma unroll
-  for (int j = 0; j < HOLD; ++j) {
-    const int i = tid + j * TPR;
-    first[j] = i < best * 32 ? lp_key_id(key[LP_JOIN_MAX - 32 + i / 32]) * 32 : 0;
-  }
-  sync();
-#pragma unroll
-  for (int j = 0; j < HOLD; ++j) {
-    const int i = tid + j * TPR;
-    const uint32_t id = first[j] + i % 32;
-    if (i < best * 32 && id < (uint32_t)shape.V && x[j] >= least) {
-      const int to = atomicAdd(&counts[w][2], 1);
-      key[to] = lp_key(x[j], id);
-    }
+  const float least = best == k ? lp_key_value(best_key[w][k - 1]) : -INFINITY;
+#pragma unroll 4
+  for (int i = tid; i < best * 32; i += TPR) {
+    const uint32_t id = lp_key_id(best_key[w][i / 32]) * 32 + i % 32;
+    const float x = dump[(int64_t)chosen[w][i / 32] * 32 + i % 32];
+    if (id < (uint32_t)shape.V && x >= least) key[atomicAdd(&counts[w][2], 1)] = lp_key(x, id);
   }
   sync();
   const int n = counts[w][2];
@@ -694,6 +682,8 @@ LpShape lp_shape(int64_t N, int64_t V, int64_t D, bool f32, int sms) {
   s.slots = (int)(most < s.pairs ? most : s.pairs);
   return s;
 }
+// Keys of one row of lp_join_kernel: the first chunks of its shares, chunks of k lists, logits of k chunks.
+int lp_join_room(int shares, int k) { return std::max(shares, 32 * k); }
 int lp_groups(const LpShape& s) { return (int)cdiv(s.col_tiles, s.group); }
 int lp_list_k(int k) { return k == 0 ? 0 : k <= 8 ? 8 : 32; }
 
