@@ -375,3 +375,44 @@ def test_refusals():
     for bad in (t.float(), t.bool()):
         with pytest.raises(TypeError):
             token_logprobs(x, bad)
+
+
+@pytest.mark.parametrize("N,V,k", [(9000, 8000, 8), (9000, 8000, 1), (9001, 30000, 20), (9000, 29999, 32), (2100, 33000, 9)])
+def test_head_alternatives_of_many_rows(N, V, k):
+    """The forms for many rows (lists kept by the epilogue, rows in several launches), on a grid (above):
+    some rows all equal, some ascending (each chunk enters the list), some descending."""
+    D = 64
+    gen = torch.Generator(device="cuda").manual_seed(N + k)
+    h = (torch.randn(N, D, device="cuda", generator=gen) * 4).round().clamp(-15, 15) / 8
+    w = (torch.randn(V, D, device="cuda", generator=gen) * 3).round().clamp(-15, 15) / 64
+    w[:, 0] = torch.arange(V, device="cuda") // 128 / 2 ** 8
+    h[:, 0] = 0
+    h[5:1000:100] = 0
+    h[7:1000:100] = 0
+    h[7:1000:100, 0] = 8
+    h[9:1000:100] = 0
+    h[9:1000:100, 0] = -8
+    t = torch.randint(-1, V, (N,), device="cuda", generator=gen)
+    h, w = h.bfloat16(), w.bfloat16()  # (257 / 256 and the like round: the definition takes them rounded)
+    r = lm_head_logprobs(h, w, t, top_k=k)
+    for a in range(0, N, 1024):
+        rows = slice(a, a + 1024)
+        x = h[rows].double() @ w.double().t()
+        check_stats(type(r)(*(o[rows] for o in r)), x, t[rows], k)
+    assert L.device_error() == 0
+
+
+def test_head_rows_of_nan():
+    """A row of hidden states that holds a NaN, in each form: NaN results, ids in range, other rows as they
+    are."""
+    for N, V, k in ((3, 500, 20), (600, 4000, 9), (9000, 8000, 8)):
+        h = torch.randn(N, 64, device="cuda").bfloat16()
+        w = torch.randn(V, 64, device="cuda").bfloat16()
+        t = torch.randint(0, V, (N,), device="cuda")
+        want = lm_head_logprobs(h, w, t, top_k=k)
+        h[1, 5] = float("nan")
+        r = lm_head_logprobs(h, w, t, top_k=k)
+        assert bool(r.logprobs[1].isnan()) and bool(r.entropy[1].isnan()) and bool(r.top_logprobs[1].isnan().all())
+        assert r.top_ids[1].tolist() == list(range(k))
+        keep = torch.arange(N, device="cuda") != 1
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(r, want))

@@ -518,11 +518,28 @@ int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const floa
 bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
 constexpr int LP_MAX_K_SPLITS = 4;
+constexpr int64_t LP_DUMP_BYTES = 256ll << 20;
+
+// How the head's forward finds the alternatives: from register lists of chunks where the rows are so many
+// that the epilogue sees a row long enough to keep its list for most chunks, or from the logits themselves,
+// written out for as many rows at a time as 256 MB hold. At V = 32000, D = 768, k = 8 lists take 119 us for
+// 2048 rows and 192 for 4096, written out 120 and 243; k = 20 lists 294 us for 4096 rows and 797 for 16384,
+// written out 251 and 1014.
+bool lp_lists(int64_t N, int64_t V, int k) {
+  return k > 0 && N * V > (k <= LP_LIST ? 2048ll * 32000 : 8192ll * 32000);
+}
+int64_t lp_ld_max(int64_t V) { return cdiv(V, 256) * 8; }  // chunks of whole tiles
+int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
+  if (k == 0 || lp_lists(N, V, k)) return N;
+  const int64_t fit = std::max<int64_t>(1, (LP_DUMP_BYTES / (lp_ld_max(V) * 128)) / 256) * 256;
+  // even steps
+  return std::min(N, cdiv(cdiv(N, cdiv(N, fit)), 256) * 256);
+}
 
 // The work buffer of the head's entries.
 struct LpWork {
   void *h_parts, *w_parts, *dx, *dx_parts;
-  float *part, *given, *dump, *sums;
+  float *part, *given, *dump, *chunk_max, *sums;
   float2* list;
   int64_t bytes;
 };
@@ -533,6 +550,7 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     p += (bytes + 255) / 256 * 256;
     return q;
   };
+  auto floats = [&](int64_t n) { return reinterpret_cast<float*>(take(n * 4)); };
   LpWork w{};
   const int64_t ldd = ulm_operand_ld(D), ldv = ulm_operand_ld(V);
   if (f32) {
@@ -544,14 +562,25 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     if (f32)
       w.dx_parts = take(3 * N * ldv * 2);
     else  // partial sums of dh or dW, whichever is split
-      w.sums = reinterpret_cast<float*>(take(LP_MAX_K_SPLITS * std::max(N, V) * D * 4));
+      w.sums = floats(LP_MAX_K_SPLITS * std::max(N, V) * D);
   } else {
-    const LpShape s = lp_shape(N, V, D, f32, lp_sms());
-    const int64_t shares = N * lp_groups(s) * s.slots * 2;
-    w.part = reinterpret_cast<float*>(take(shares * 16));
-    w.list = reinterpret_cast<float2*>(take(shares * k * 8));
-    w.dump = reinterpret_cast<float*>(take(shares * k * 128));
-    w.given = reinterpret_cast<float*>(take(N * 4));
+    const int64_t rows = lp_rows_at_once(N, V, k);
+    // the shares of the rows of one launch: all of them, but for the last one's fewer rows
+    int64_t shares = 0;
+    for (const int64_t n : {rows, N % rows}) {
+      if (n == 0) continue;
+      const LpShape s = lp_shape(n, V, D, f32, lp_sms());
+      shares = std::max(shares, n * lp_groups(s) * s.slots * 2);
+    }
+    w.part = floats(shares * 4);
+    w.given = floats(rows);
+    if (lp_lists(N, V, k)) {
+      w.list = reinterpret_cast<float2*>(take(shares * k * 8));
+      w.dump = floats(shares * k * 32);
+    } else if (k > 0) {
+      w.dump = floats(rows * lp_ld_max(V) * 32);
+      w.chunk_max = floats(rows * lp_ld_max(V));
+    }
   }
   w.bytes = p - static_cast<char*>(base);
   return w;
@@ -616,32 +645,47 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
   ULM_REQUIRE(logprobs && entropy && work, "null pointer argument");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f32 = prec == ULM_PREC_FP32;
-  const LpShape s = lp_shape(N, V, D, f32, lp_sms());
   const LpWork w = lp_work(work, N, V, D, top_k, false, f32);
-  ULM_REQUIRE(lp_groups(s) * s.slots * 2 <= LP_JOIN_MAX, "too many column groups");
+  const bool lists = lp_lists(N, V, top_k), dump = top_k > 0 && !lists;
+  const int64_t step = lp_rows_at_once(N, V, top_k), es = f32 ? 4 : 2;
   CUtensorMap th, tw, to;
   memset(&to, 0, sizeof(to));
-  if (int rc = lp_operand(&th, h_op, ld_h, N, D, f32, w.h_parts, st)) return rc;
   if (int rc = lp_operand(&tw, w_op, ld_w, V, D, f32, w.w_parts, st)) return rc;
-  LpArgs a{};
-  a.tokens = tokens;
-  a.part = w.part;
-  a.list = w.list;
-  a.dump = w.dump;
-  a.given = w.given;
-  a.k = top_k;
-  a.groups = lp_groups(s);
-  const int K = lp_list_k(top_k);
-  const int rc = K == 0   ? lp_launch<LP_STATS, 0, false>(th, tw, to, s, a, st)
-                 : K == 8 ? lp_launch<LP_STATS, 8, false>(th, tw, to, s, a, st)
-                          : lp_launch<LP_STATS, 32, false>(th, tw, to, s, a, st);
-  if (rc) return rc;
-  const int room = top_k > 0 ? lp_join_room(lp_groups(s) * s.slots * 2, top_k) : 0;
-  if (N <= 4 * (int64_t)lp_sms())
-    return launch_pdl(lp_join_kernel<128>, dim3((unsigned)N), dim3(128), (size_t)room * 12, st, s, a, logprobs, entropy,
-                      stats, top_ids, top_logprobs, room);
-  return launch_pdl(lp_join_kernel<32>, dim3((unsigned)cdiv(N, LP_JOIN_ROWS)), dim3(32 * LP_JOIN_ROWS),
-                    (size_t)room * 12 * LP_JOIN_ROWS, st, s, a, logprobs, entropy, stats, top_ids, top_logprobs, room);
+  for (int64_t r0 = 0; r0 < N; r0 += step) {
+    const int64_t n = std::min(step, N - r0);
+    const LpShape s = lp_shape(n, V, D, f32, lp_sms());
+    const int shares = lp_groups(s) * s.slots * 2;  // of a row
+    ULM_REQUIRE(shares <= LP_JOIN_MAX, "too many column groups");
+    if (int rc = lp_operand(&th, static_cast<const char*>(h_op) + r0 * ld_h * es, ld_h, n, D, f32, w.h_parts, st)) return rc;
+    if (dump)
+      ULM_REQUIRE(make_epi_tmap(&to, EPI_MODE_WARP, w.dump, ULM_F32, V, n, 1, lp_ld_max(V) * 32, 0),
+                  "no tensor map of the logits");
+    LpArgs a{};
+    a.tokens = tokens + r0;
+    a.part = w.part;
+    a.list = w.list;
+    a.dump = w.dump;
+    a.given = w.given;
+    a.k = lists ? top_k : 0;
+    a.groups = lp_groups(s);
+    a.chunk_max = w.chunk_max;
+    a.ld_max = lp_ld_max(V);
+    if (int rc = dump    ? lp_launch<LP_DUMP, 0, false>(th, tw, to, s, a, st)
+                 : !lists ? lp_launch<LP_STATS, 0, false>(th, tw, to, s, a, st)
+                 : top_k <= LP_LIST ? lp_launch<LP_STATS, LP_LIST, false>(th, tw, to, s, a, st)
+                                    : lp_launch<LP_STATS, LP_LONG_LIST, false>(th, tw, to, s, a, st))
+      return rc;
+    a.k = top_k;
+    const int room = top_k == 0 ? 0 : lp_join_room(lists ? shares : 0, top_k);
+    const bool wide = dump || n <= 4 * (int64_t)lp_sms();
+    const int rc = launch_pdl(dump ? lp_join_kernel<128, true> : wide ? lp_join_kernel<128, false> : lp_join_kernel<32, false>,
+                              dim3((unsigned)(wide ? n : cdiv(n, LP_JOIN_ROWS))), dim3(wide ? 128 : 32 * LP_JOIN_ROWS),
+                              (size_t)room * 12 * (wide ? 1 : LP_JOIN_ROWS), st, s, a, logprobs + r0, entropy + r0,
+                              stats ? stats + 2 * r0 : nullptr, top_ids ? top_ids + r0 * top_k : nullptr,
+                              top_logprobs ? top_logprobs + r0 * top_k : nullptr, room);
+    if (rc) return rc;
+  }
+  return ULM_OK;
 }
 
 extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,

@@ -4,9 +4,12 @@
 //
 // LP_STATS keeps, for each row, the running maximum, sum of exponentials and entropy sum of the softmax in
 // registers from tile to tile; an epilogue thread owns half of a row's columns, in chunks of 32 logits.
-// For the k best alternatives it keeps a sorted list of its k best chunks, by their maxima, and writes a
-// chunk that enters the list to the place of the one that leaves it (about k ln(chunks / k) times a row):
-// the k best logits lie in the k best chunks, so one comparison serves 32 logits.
+// The k best logits of a row lie in its k best chunks, by their maxima, so the alternatives take one
+// comparison for 32 logits. For many rows an epilogue thread keeps a sorted list of the k best chunks of its
+// share and writes a chunk that enters the list to the place of the one that leaves it (about
+// k ln(chunks / k) times). LP_DUMP, for few rows, where most chunks of the short shares would enter, writes
+// all logits and the maxima of the chunks, and lp_join_kernel picks (2048 x 32000 x 768, k = 20: lists 188
+// us, written out 125; 16384 rows: 797 and 1014; no alternatives: 75 and 561).
 // LP_GRAD writes the logits' gradient ([v = t] a - p (a + b (log p + H))) in the operand type of the
 // products that follow.
 //
@@ -30,7 +33,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int LP_MAX_TOP = 32;  // top_k of the entries
 
-enum { LP_STATS = 0, LP_GRAD = 1 };
+enum { LP_STATS = 0, LP_GRAD = 1, LP_DUMP = 2 };
 constexpr int LPM_STAGES = 5;
 constexpr int LPM_SLOTS = 2;  // 4 KB staging tiles of an epilogue warp (LP_GRAD)
 constexpr uint32_t LPM_HALF_BYTES = 128 * 64 * 2;  // a CTA's 128 rows of one operand, 64 k values
@@ -83,6 +86,10 @@ struct LpArgs {
   float* dump;
   float* given;
   int k;
+  // LP_DUMP: besides part and given, the largest logit of each chunk of 32 columns in
+  // chunk_max[row * ld_max + column / 32] (the logits themselves go through the output's tensor map)
+  float* chunk_max;
+  int64_t ld_max;
   int groups;
   // LP_GRAD
   const float* stats;
@@ -114,6 +121,7 @@ __device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* st
 template <int K>
 struct LpRun {
   float m, m2, s, u;  // maximum (at least -1e30), m log2 e, sum 2^(x log2 e - m2), sum 2^(.) (.)
+  float last;         // maximum of the chunk added last
   float v[K > 0 ? K : 1];
   int id[K > 0 ? K : 1];
 
@@ -138,6 +146,7 @@ struct LpRun {
     float lm = fmaxf(x[0], x[1]);
 #pragma unroll
     for (int i = 2; i < 32; i += 2) lm = fmaxf(lm, fmaxf(x[i], x[i + 1]));
+    last = lm;
     if (K > 0) {
       if (lm > v[K - 1]) {
         const int place = id[K - 1] & 31, mine = col0 | place;
@@ -223,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tma_h);
     tma_prefetch_desc(&tma_w);
-    if (MODE == LP_GRAD) tma_prefetch_desc(&tma_out);
+    if (MODE != LP_STATS) tma_prefetch_desc(&tma_out);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -338,9 +347,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
     LpCoef c;
     float* dump = nullptr;  // the chunks of this thread's share
     int64_t share = 0;
-    if (MODE == LP_STATS) run.reset(false, 0);
+    if (MODE != LP_GRAD) run.reset(false, 0);
     auto flush = [&]() {
-      if (MODE != LP_STATS || at_rb < 0 || !live) return;
+      if (MODE == LP_GRAD || at_rb < 0 || !live) return;
       *reinterpret_cast<float4*>(args.part + 4 * share) = make_float4(run.m, run.s, run.u, 0.f);
       if (K > 0) {
 #pragma unroll
@@ -356,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         at_g = tile.g;
         row = (int64_t)tile.rb * 256 + (int64_t)rank * 128 + quad * 32 + lane;
         live = row < shape.N;
-        if (MODE == LP_STATS) {
+        if (MODE != LP_GRAD) {
           const int slot = pair - lp_pair_of(shape, lp_row_first(shape, at_g, at_rb));
           share = ((row * args.groups + at_g) * shape.slots + slot) * 2 + half;
           dump = args.dump + share * args.k * 32;
@@ -375,10 +384,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
       const int col_base = tile.ct * 256 + half * 128;
       const bool rows_here = __any_sync(0xffffffffu, live);
       const int chunks = rows_here ? min(4, (shape.V - col_base + 31) / 32) : 0;
-      if (MODE == LP_STATS) {
+      if (MODE != LP_GRAD) {
+        uint32_t ra[32], rb[32];
+        float4 cmax = make_float4(0.f, 0.f, 0.f, 0.f);
         // a list of 32 leaves no registers for the next chunk's load ahead
         constexpr bool AHEAD = K <= 8;
-        uint32_t ra[32], rb[32];
         if (AHEAD && chunks > 0) tmem_ld_32x32_issue(taddr, ra);
         auto one = [&](uint32_t (&r)[32], uint32_t (&next)[32], int ch) {
           const int col0 = col_base + 32 * ch;
@@ -396,6 +406,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
               if (col0 + i == (int)tok) g = x[i];
             args.given[row] = g;
           }
+          if (MODE == LP_DUMP) {
+            (ch == 0 ? cmax.x : ch == 1 ? cmax.y : ch == 2 ? cmax.z : cmax.w) = run.last;
+            uint8_t* out = slots + (n % LPM_SLOTS) * 4096;
+            ++n;
+            if (lane == 0) bulk_wait_group_read<LPM_SLOTS - 1>();  // the store before last has read its slot
+            __syncwarp();
+            stage_write<true, 32>(out, lane, 0, x);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&tma_out, out, col0, tile.rb * 256 + (int)rank * 128 + quad * 32, 0);
+              bulk_commit_group();
+            }
+          }
           __syncwarp();
         };
         if (AHEAD) {
@@ -408,6 +432,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
 #pragma unroll 1
           for (int ch = 0; ch < chunks; ++ch) one(ra, rb, ch);
         }
+        if (MODE == LP_DUMP && live && chunks > 0)  // rows of chunk_max are whole tiles long
+          *reinterpret_cast<float4*>(args.chunk_max + row * args.ld_max + col_base / 32) = cmax;
       } else {
         constexpr int CW = F32 ? 32 : 64;  // columns of a staged chunk of 128 bytes a row
         const int nch = rows_here ? min(128 / CW, (shape.V - col_base + CW - 1) / CW) : 0;
@@ -479,9 +505,12 @@ __device__ __forceinline__ uint32_t lp_key_id(uint64_t k) { return 0xFFFFFFFFu -
 // hold one of the row's k best chunks, and of the row's logits only those in its k best chunks (a chunk
 // with k better ones ahead of it, in the order of maximum and column, has k better logits ahead of all of
 // its own). Each of the three choices is a rank among at most 1024 keys, about k of them in the last two.
+// DUMP: the logits are there whole, with the maximum of each chunk: the best chunks are looked for among
+// those not under the k-th largest of 64 groups' maxima.
 constexpr int LP_JOIN_MAX = 1024;  // shares of one row, and chunks or logits to choose from
+constexpr int LP_JOIN_GROUPS = 64;
 constexpr int LP_JOIN_ROWS = 2;    // rows of a CTA when a warp has a row
-template <int TPR>
+template <int TPR, bool DUMP>
 __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     lp_join_kernel(const LpShape shape, const LpArgs args, float* __restrict__ logprobs, float* __restrict__ entropy,
                    float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs,
@@ -493,6 +522,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
   __shared__ int counts[ROWS][3];
   __shared__ uint64_t bound[ROWS];
   __shared__ float4 wred[TPR / 32];
+  __shared__ float gmax[DUMP ? TPR : 1];
+  __shared__ float thr_s;
   pdl_enter();
   const int tid = threadIdx.x % TPR, w = threadIdx.x / TPR;
   const int64_t row = (int64_t)blockIdx.x * ROWS + w;
@@ -535,7 +566,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
   for (int i = tid; i < all; i += TPR) {
     if (!there(i)) continue;
     const float4 p = part[i];
-    if (k > 0) {  // the share's first chunk
+    if (!DUMP && k > 0) {  // the share's first chunk
       const float2 e = list[(int64_t)i * k];
       const int id = __float_as_int(e.y);
       if (id >= 0) {
@@ -583,6 +614,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
       if (r < k) f(c, r);
     }
   };
+  int best = 0;
+  if (!DUMP) {
   sync();
   const int heads = counts[w][0], lists = min(heads, k);
   rank(heads, [&](int c, int r) {
@@ -606,9 +639,82 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     }
   }
   sync();
-  const int chunks = counts[w][1], best = min(chunks, k);
+  const int chunks = counts[w][1];
+  best = min(chunks, k);
   rank(chunks, [&](int c, int r) { chosen[w][r] = c; });
   sync();
+  } else {
+    const int chunks = (shape.V + 31) / 32;
+    const float* cm = args.chunk_max + row * args.ld_max;
+    best = min(chunks, k);
+    float g = -INFINITY;
+#pragma unroll 4
+    for (int i = tid; i < chunks; i += TPR) g = fmaxf(g, cm[i]);
+    gmax[tid] = g;
+    if (tid == 0) thr_s = -INFINITY;
+    sync();
+    if (tid < LP_JOIN_GROUPS) {
+      float mine = gmax[tid];
+#pragma unroll
+      for (int j = 1; j < TPR / LP_JOIN_GROUPS; ++j) mine = fmaxf(mine, gmax[tid + j * LP_JOIN_GROUPS]);
+      gmax[tid] = mine;
+    }
+    sync();
+    if (tid < LP_JOIN_GROUPS) {
+      const float mine = gmax[tid];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < LP_JOIN_GROUPS; ++j) r += (gmax[j] > mine || (gmax[j] == mine && j < tid)) ? 1 : 0;
+      if (r == k - 1) thr_s = mine;
+    }
+    sync();
+    const float thr = thr_s;
+#pragma unroll 4
+    for (int i = tid; i < chunks; i += TPR) {
+      const float x = cm[i];
+      if (x >= thr) {
+        const int to = atomicAdd(&counts[w][1], 1);
+        if (to < room) {
+          key[to] = lp_key(x, (uint32_t)i);
+          at[to] = i;
+        }
+      }
+    }
+    sync();
+    const int n = counts[w][1];
+    if (n <= room) {
+      best = min(n, k);  // fewer only where a chunk is all NaN
+      rank(n, [&](int c, int r) { chosen[w][r] = c; });
+      sync();
+    } else {
+      // many equal maxima: the best one after the last, k times
+      uint64_t last = ~0ull;
+      for (int j = 0; j < best; ++j) {
+        uint64_t top = 0;
+        for (int i = tid; i < chunks; i += TPR) {
+          const uint64_t kk = lp_key(cm[i], (uint32_t)i);
+          if (kk < last && kk > top) top = kk;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, top, o);
+          top = other > top ? other : top;
+        }
+        sync();
+        if ((tid & 31) == 0) best_key[w][tid >> 5] = top;
+        sync();
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) top = best_key[w][i] > top ? best_key[w][i] : top;
+        last = top;
+        if (tid == 0) {
+          key[j] = top;
+          at[j] = (int)lp_key_id(top);
+          chosen[w][j] = j;
+        }
+      }
+      sync();
+    }
+  }
   // the best chunks; the last one's maximum bounds the k-th best logit from below
   int mine_at = 0;
   if (tid < best) {
@@ -622,7 +728,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
 #pragma unroll 4
   for (int i = tid; i < best * 32; i += TPR) {
     const uint32_t id = lp_key_id(best_key[w][i / 32]) * 32 + i % 32;
-    const float x = dump[(int64_t)chosen[w][i / 32] * 32 + i % 32];
+    const float x = DUMP ? (id < (uint32_t)shape.V ? args.dump[row * args.ld_max * 32 + id] : -INFINITY)
+                         : dump[(int64_t)chosen[w][i / 32] * 32 + i % 32];
     if (id < (uint32_t)shape.V && x >= least) key[atomicAdd(&counts[w][2], 1)] = lp_key(x, id);
   }
   sync();
@@ -685,7 +792,7 @@ LpShape lp_shape(int64_t N, int64_t V, int64_t D, bool f32, int sms) {
 // Keys of one row of lp_join_kernel: the first chunks of its shares, chunks of k lists, logits of k chunks.
 int lp_join_room(int shares, int k) { return std::max(shares, 32 * k); }
 int lp_groups(const LpShape& s) { return (int)cdiv(s.col_tiles, s.group); }
-int lp_list_k(int k) { return k == 0 ? 0 : k <= 8 ? 8 : 32; }
+constexpr int LP_LIST = 8, LP_LONG_LIST = 32;  // chunks in a register list
 
 template <int MODE, int K, bool F32>
 int lp_launch(const CUtensorMap& th, const CUtensorMap& tw, const CUtensorMap& to, const LpShape& s, const LpArgs& a,
