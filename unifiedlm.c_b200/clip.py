@@ -82,10 +82,8 @@ def clip_grads(grads, max_norm, out=None):
     if len(outs) != len(grads):
         raise ValueError(f"{len(grads)} gradients and {len(outs)} outputs")
     for g, o in zip(grads, outs) if outs is not grads else ():
-        if o.shape != g.shape:
-            raise ValueError(f"output {tuple(o.shape)} for a gradient {tuple(g.shape)}")
-        if o.device != g.device:
-            raise ValueError(f"output on {o.device} for a gradient on {g.device}")
+        if o.shape != g.shape or o.get_device() != g.get_device():
+            raise ValueError(f"output {tuple(o.shape)} on {o.device} for a gradient {tuple(g.shape)} on {g.device}")
     if not grads:
         return torch.tensor(0.0)
     with torch.no_grad():

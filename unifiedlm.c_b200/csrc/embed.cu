@@ -349,19 +349,20 @@ __global__ void __launch_bounds__(EMB_THREADS)
   }
 }
 
-// CTA (c, column block of 32): if a run begins in chunk c and goes on, the sum of its shares: warp w
+// CTA (c, block of 32 NV columns): if a run begins in chunk c and goes on, the sum of its shares: warp w
 // adds every eighth one, then the warps' sums are added in order.
+template <int NV>
 __global__ void __launch_bounds__(EMB_THREADS)
     embed_join_kernel(const int* __restrict__ key, const float* __restrict__ part, void* __restrict__ dw, int dw_dtype,
                       int N, int V, int64_t D, float scale) {
   pdl_enter();
-  __shared__ float red[EMB_THREADS / 32][32];
+  __shared__ float red[EMB_THREADS / 32][32 * NV];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = blockIdx.x, i0 = c * EMB_CHUNK, last = i0 + EMB_CHUNK - 1;
   if (last + 1 >= N) return;
-  const int k = key[last];
-  if (k >= V || key[last + 1] != k) return;                   // no run goes on
-  if (key[i0] == k && i0 > 0 && key[i0 - 1] == k) return;     // it began in an earlier chunk
+  const int k = key[last], after = key[last + 1], begin = key[i0], before = i0 > 0 ? key[i0 - 1] : -1;
+  if (k >= V || after != k) return;            // no run goes on
+  if (begin == k && before == k) return;       // it began in an earlier chunk
   // chunks c + 1 .. c + more begin with entries of the same run
   const int64_t chunks = (N + EMB_CHUNK - 1) / EMB_CHUNK;
   int64_t more = 0;
@@ -375,19 +376,34 @@ __global__ void __launch_bounds__(EMB_THREADS)
       break;
     }
   }
-  const int64_t d = (int64_t)blockIdx.y * 32 + lane;
-  float acc = 0.f;
+  const int64_t d = ((int64_t)blockIdx.y * 32 + lane) * NV;
+  float acc[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = 0.f;
   if (d < D) {
 #pragma unroll 8
-    for (int64_t j = w; j <= more; j += EMB_THREADS / 32) acc += part[(j == 0 ? 2 * c + 1 : 2 * (c + j)) * D + d];
+    for (int64_t j = w; j <= more; j += EMB_THREADS / 32) {
+      const float* p = part + (j == 0 ? 2 * c + 1 : 2 * (c + j)) * D + d;
+      float x[NV];
+      if (NV == 4)
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+      else
+        x[0] = p[0];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) acc[i] += x[i];
+    }
   }
-  red[w][lane] = acc;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) red[w][lane + 32 * i] = acc[i];
   __syncthreads();
   if (w == 0 && d < D) {
-    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < EMB_THREADS / 32; ++i) s += red[i][lane];
-    emb_store(dw, dw_dtype, (int64_t)k * D + d, s * scale);
+    for (int i = 0; i < NV; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < EMB_THREADS / 32; ++j) s += red[j][lane + 32 * i];
+      emb_store(dw, dw_dtype, (int64_t)k * D + d + i, s * scale);
+    }
   }
 }
 
@@ -429,7 +445,8 @@ int emb_sums(const EmbWork& w, const int* key, const int* pos, const void* dy, v
                           dw_dtype, w.part, (int)N, (int)V, D, (int)cols, scale))
     return rc;
   if (chunks < 2) return ULM_OK;
-  return launch_pdl(embed_join_kernel, dim3((unsigned)(chunks - 1), (unsigned)cdiv(D, 32)), dim3(EMB_THREADS), 0, st, key,
+  return launch_pdl(vec ? embed_join_kernel<4> : embed_join_kernel<1>,
+                    dim3((unsigned)(chunks - 1), (unsigned)cdiv(D, vec ? 128 : 32)), dim3(EMB_THREADS), 0, st, key,
                     static_cast<const float*>(w.part), dw, dw_dtype, (int)N, (int)V, D, scale);
 }
 

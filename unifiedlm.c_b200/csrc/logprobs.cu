@@ -42,8 +42,9 @@ __device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b) {
 // NV more logits into a thread's statistics: the largest and the smallest first. Where a logit is below
 // -1e30 (-inf, or the type's lowest value, is a mask) its term is left out: 2^(.) is 0, but (.) may be
 // -inf.
+// Returns the largest, or +inf once the sum is NaN.
 template <int NV>
-__device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
+__device__ __forceinline__ float lp_add(LpStat& st, const float (&x)[NV]) {
   float hi = x[0], lo = x[0];
 #pragma unroll
   for (int i = 1; i < NV; ++i) {
@@ -58,7 +59,7 @@ __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
       st.s += e;
       st.u = e > 0.f ? fmaf(e, d, st.u) : st.u;
     }
-    return;
+    return st.s == st.s ? hi : INFINITY;
   }
   float s1 = 0.f, u1 = 0.f;
 #pragma unroll
@@ -69,6 +70,7 @@ __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[NV]) {
   }
   st.s += s1;
   st.u += u1;
+  return st.s == st.s ? hi : INFINITY;
 }
 
 template <typename T>
@@ -120,6 +122,15 @@ struct LpVec<__nv_bfloat16> {
   }
 };
 
+// Pieces of a thread in flight: 16 values.
+template <typename T>
+constexpr int LP_UNROLL = 16 / LpVec<T>::N;
+// CTAs an SM, by the registers that the batches leave (8192 x 32000 bf16: 6 CTAs 99 us, 5 106; fp32 is
+// faster with 5)
+template <typename T>
+constexpr int LP_CTAS = LpVec<T>::N == 8 ? 6 : 5;
+constexpr int LP_KEPT = 16;  // batches of a thread whose maxima are kept for the second look
+
 // Elements before the first 16-byte boundary at p, at most n.
 template <typename T>
 __device__ __forceinline__ int lp_head(const T* p, int n) {
@@ -127,39 +138,58 @@ __device__ __forceinline__ int lp_head(const T* p, int n) {
   return h < n ? h : n;
 }
 
-// f(id, values) over logits c0 .. c1 of a row, four 16-byte pieces at a time (16 fp32 or 32 bf16 logits, all
-// loaded before the first is used) from the first 16-byte boundary, one piece at a time where fewer are
-// left, and one logit at a time at the two ends.
-template <typename T, typename F>
-__device__ __forceinline__ void lp_for_each(const T* row, int c0, int c1, F&& f) {
-  constexpr int NV = LpVec<T>::N, U = 4;
+// f(batch, ids, values) over logits c0 .. c1 of a row, from its first 16-byte boundary in batches of U 16-byte
+// pieces a thread (batch 0, 1, ... of the thread), loaded while the ones before are used; batch -1 for the
+// pieces and, at the two ends, the logits that are left. AGAIN: a later look, at the batches that
+// want(batch) names and at what is left.
+template <typename T, int U, bool AGAIN, typename W, typename F>
+__device__ __forceinline__ void lp_for_each(const T* row, int c0, int c1, W&& want, F&& f) {
+  constexpr int NV = LpVec<T>::N;
   const int n = c1 - c0, head = lp_head(row + c0, n), nvec = (n - head) / NV, tail0 = c0 + head + nvec * NV;
   const uint4* body = reinterpret_cast<const uint4*>(row + c0 + head);
   auto one = [&](int id) {
     const float x[1] = {lp_load(row + id)};
     const int ids[1] = {id};
-    f(ids, x);
+    f(-1, ids, x);
   };
   if ((int)threadIdx.x < head) one(c0 + (int)threadIdx.x);
-  int i = threadIdx.x;
-  for (; i + (U - 1) * LP_THREADS < nvec; i += U * LP_THREADS) {
+  uint4 ahead[U];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (i + j * LP_THREADS < nvec) ahead[j] = body[i + j * LP_THREADS];
+  };
+  if (!AGAIN) load(threadIdx.x);
+  int batch = 0;
+  for (int i = threadIdx.x; i < nvec; i += U * LP_THREADS, ++batch) {
+    const bool whole = i + (U - 1) * LP_THREADS < nvec;
+    if (AGAIN) {
+      if (whole && !want(batch)) continue;
+      load(i);
+    }
     uint4 q[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) q[j] = body[i + j * LP_THREADS];
-    float x[U * NV];
-    int ids[U];
+    for (int j = 0; j < U; ++j) q[j] = ahead[j];
+    if (!AGAIN) load(i + U * LP_THREADS);
+    if (whole) {
+      float x[U * NV];
+      int ids[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      LpVec<T>::unpack(q[j], x + j * NV);
-      ids[j] = c0 + head + (i + j * LP_THREADS) * NV;
+      for (int j = 0; j < U; ++j) {
+        LpVec<T>::unpack(q[j], x + j * NV);
+        ids[j] = c0 + head + (i + j * LP_THREADS) * NV;
+      }
+      f(batch, ids, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < U - 1; ++j) {
+        if (i + j * LP_THREADS >= nvec) break;
+        float x[NV];
+        LpVec<T>::unpack(q[j], x);
+        const int ids[1] = {c0 + head + (i + j * LP_THREADS) * NV};
+        f(-1, ids, x);
+      }
     }
-    f(ids, x);
-  }
-  for (; i < nvec; i += LP_THREADS) {
-    float x[NV];
-    LpVec<T>::unpack(body[i], x);
-    const int ids[1] = {c0 + head + i * NV};
-    f(ids, x);
   }
   if (tail0 + (int)threadIdx.x < c1) one(tail0 + (int)threadIdx.x);
 }
@@ -188,20 +218,22 @@ __device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* red) {
 }
 
 // One cluster of `split` CTAs per row, each with an equal run of its columns. A CTA makes one pass over
-// its logits for the statistics and, for the alternatives, a second one out of L1 and L2 that compares with
-// a threshold: the k-th largest of 64 groups' maxima bounds the k-th best logit of the run from below, and
-// only about k logits reach it. The cluster's first CTA joins the runs. Bound by the pass over HBM for
+// its logits for the statistics and, for the alternatives, a second look at those batches whose maximum
+// reaches a threshold: the k-th largest of 64 groups' maxima bounds the k-th best logit of the run from
+// below, and only about k logits reach it. The cluster's first CTA joins the runs. Bound by the pass over HBM for
 // many rows (4096 x 32000 bf16: 63 us, 4.1 TB/s), by latency for few: a row of 32000 split over 8 CTAs takes
 // 10 us, on one CTA 15.5 us.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS)
+__global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
     lp_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens,
                    float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ stats,
                    int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int V, int k, int split) {
-  __shared__ LpStat part[LP_THREADS / 32];
-  __shared__ LpStat runs[LP_MAX_SPLIT];                    // of the cluster's CTAs (first CTA)
+  __shared__ float wmax[LP_THREADS / 32];
+  __shared__ float2 wsum[LP_THREADS / 32];
+  __shared__ alignas(16) LpStat runs[LP_MAX_SPLIT];                    // of the cluster's CTAs (first CTA)
   __shared__ uint64_t best[LP_MAX_SPLIT * LP_MAX_TOP];     // their alternatives, 0 for none (first CTA)
   __shared__ float gmax[LP_GROUPS];
+  __shared__ float kept[LP_KEPT * LP_THREADS];
   __shared__ float thr_s;
   __shared__ uint64_t cand[LP_CAP];
   __shared__ uint64_t red[LP_THREADS / 32];
@@ -213,7 +245,12 @@ __global__ void __launch_bounds__(LP_THREADS)
   const T* row = x + r * ld;
   const int c0 = (int)((int64_t)V * rank / split), c1 = (int)((int64_t)V * (rank + 1) / split);
   LpStat st{LP_LEAST, __fmul_rn(LP_LEAST, LOG2E), 0.f, 0.f};
-  lp_for_each(row, c0, c1, [&](const auto&, const auto& v) { lp_add(st, v); });
+  constexpr int U = LP_UNROLL<T>;
+  auto all_of_them = [](int) { return true; };
+  lp_for_each<T, U, false>(row, c0, c1, all_of_them, [&](int batch, const auto&, const auto& v) {
+    const float hi = lp_add(st, v);
+    if (k > 0 && batch >= 0 && batch < LP_KEPT) kept[batch * LP_THREADS + tid] = hi;
+  });
   if (k > 0) {
     // the maxima of the groups of LP_THREADS / LP_GROUPS neighbouring threads
     float g = st.m;
@@ -221,19 +258,30 @@ __global__ void __launch_bounds__(LP_THREADS)
     for (int o = LP_THREADS / LP_GROUPS / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
     if (tid % (LP_THREADS / LP_GROUPS) == 0) gmax[tid / (LP_THREADS / LP_GROUPS)] = g;
   }
+  // the CTA's maximum, then the sums about it
+  float hi = st.m;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const LpStat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.m2, o),
-                       __shfl_xor_sync(0xffffffffu, st.s, o), __shfl_xor_sync(0xffffffffu, st.u, o)};
-    st = lp_merge(st, other);
-  }
-  if (lane == 0) part[wp] = st;
+  for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  if (lane == 0) wmax[wp] = hi;
   if (tid == 0) count = 0;
   __syncthreads();
-  if (tid == 0) {
-    LpStat all = part[0];
 #pragma unroll
-    for (int w = 1; w < LP_THREADS / 32; ++w) all = lp_merge(all, part[w]);
+  for (int w = 0; w < LP_THREADS / 32; ++w) hi = fmaxf(hi, wmax[w]);
+  st.raise(hi);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+    st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
+  }
+  if (lane == 0) wsum[wp] = make_float2(st.s, st.u);
+  __syncthreads();
+  if (tid == 0) {
+    LpStat all{st.m, st.m2, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < LP_THREADS / 32; ++w) {
+      all.s += wsum[w].x;
+      all.u += wsum[w].y;
+    }
     if (rank == 0) {
       runs[0] = all;
     } else {
@@ -260,11 +308,13 @@ __global__ void __launch_bounds__(LP_THREADS)
     // above it are then taken, and masked ones in the order of their ids where they are fewer than k.
     const float thr = thr_s;
     const bool few = thr <= LP_LEAST;
-    lp_for_each(row, c0, c1, [&](const auto& ids, const auto& v) {
+    auto reaches = [&](float v) { return few ? !(v <= thr) : !(v < thr); };
+    auto want = [&](int batch) { return batch >= LP_KEPT || reaches(kept[batch * LP_THREADS + tid]); };
+    lp_for_each<T, U, true>(row, c0, c1, want, [&](int, const auto& ids, const auto& v) {
       constexpr int NV = (int)(sizeof(v) / sizeof(float)), NI = (int)(sizeof(ids) / sizeof(int));
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (few ? !(v[i] <= thr) : !(v[i] < thr)) {
+        if (reaches(v[i])) {
           const int at = atomicAdd(&count, 1);
           if (at < LP_CAP) cand[at] = lp_key(v[i], (uint32_t)(ids[i / (NV / NI)] + i % (NV / NI)));
         }
@@ -287,7 +337,7 @@ __global__ void __launch_bounds__(LP_THREADS)
       uint64_t last = ~0ull;
       for (int j = 0; j < k; ++j) {
         uint64_t top = 0;
-        lp_for_each(row, c0, c1, [&](const auto& ids, const auto& v) {
+        lp_for_each<T, U, true>(row, c0, c1, all_of_them, [&](int, const auto& ids, const auto& v) {
           constexpr int NV = (int)(sizeof(v) / sizeof(float)), NI = (int)(sizeof(ids) / sizeof(int));
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -360,13 +410,6 @@ __global__ void __launch_bounds__(LP_THREADS)
   }
 }
 
-__device__ __forceinline__ float lp_dlogit(const LpCoef& c, float x, int64_t v) {
-  const float logp = (x - c.base) - c.logs;
-  const float p = fast_exp2(logp * LOG2E);
-  const float d = p == 0.f ? 0.f : p * fmaf(c.b, logp, c.c0);
-  return (v == c.t ? c.a : 0.f) - d;
-}
-
 template <typename T>
 __device__ __forceinline__ void lp_store(T* p, float v);
 template <>
@@ -397,15 +440,14 @@ __global__ void __launch_bounds__(LP_THREADS)
   const bool same = ((reinterpret_cast<uintptr_t>(src) ^ reinterpret_cast<uintptr_t>(dst)) & 15) == 0;
   const int head = same ? lp_head(src, n) : n, nvec = (n - head) / NV;
 #pragma unroll 4
-  for (int i = tid; i < head; i += LP_THREADS) lp_store(dst + i, lp_dlogit(c, lp_load(src + i), c0 + i));
+  for (int i = tid; i < head; i += LP_THREADS) lp_store(dst + i, c.others(lp_load(src + i)));
   const uint4* sv = reinterpret_cast<const uint4*>(src + head);
   uint4* dv = reinterpret_cast<uint4*>(dst + head);
   auto piece = [&](const uint4& q, int i) {
     float v[NV];
     LpVec<T>::unpack(q, v);
-    const int id = c0 + head + i * NV;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = lp_dlogit(c, v[j], id + j);
+    for (int j = 0; j < NV; ++j) v[j] = c.others(v[j]);
     dv[i] = LpVec<T>::pack(v);
   };
   int i = tid;
@@ -418,7 +460,9 @@ __global__ void __launch_bounds__(LP_THREADS)
   }
   for (; i < nvec; i += LP_THREADS) piece(sv[i], i);
   const int tail = head + nvec * NV + tid;
-  if (tail < n) lp_store(dst + tail, lp_dlogit(c, lp_load(src + tail), c0 + tail));
+  if (tail < n) lp_store(dst + tail, c.others(lp_load(src + tail)));
+  __syncthreads();
+  if (tid == 0 && c.t >= c0 && c.t < c0 + n) lp_store(dst + (c.t - c0), c.others(lp_load(src + (c.t - c0))) + c.a);
 }
 
 int lp_sms() {
@@ -426,12 +470,13 @@ int lp_sms() {
   return dev >= 0 ? sm_count(dev) : 148;
 }
 
-// A row is split over as many CTAs as fit on the GPU at once (4 of them an SM), each with 2048 logits at
+// A row is split over as many CTAs as fit on the GPU at once, each with 2048 logits at
 // least.
 int lp_rows_fwd(const void* x, int dtype, int64_t ld, const int64_t* tokens, float* logprobs, float* entropy,
                 float* stats, int64_t* top_ids, float* top_logprobs, int64_t N, int64_t V, int k, cudaStream_t st) {
   int split = 1;
-  while (split < LP_MAX_SPLIT && N * split * 2 <= 4 * (int64_t)lp_sms() && V / (split * 2) >= 2048) split *= 2;
+  const int ctas = dtype == ULM_F32 ? LP_CTAS<float> : LP_CTAS<__nv_bfloat16>;
+  while (split < LP_MAX_SPLIT && N * split * 2 <= ctas * (int64_t)lp_sms() && V / (split * 2) >= 2048) split *= 2;
   ULM_REQUIRE(N * split < (1ll << 31), "extent too large");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(N * split));

@@ -98,21 +98,31 @@ struct LpArgs {
   const float* dentropy;
 };
 
-// The backward's factors of one row: dx_v = ([v = t] a) - p_v (a + b (log p_v + H)).
+// The backward's factors of one row: dx_v = [v = t] a - p_v (a + b (log p_v + H)), in base 2 as the
+// statistics are: p_v = 2^l, l = (x_v log2 e - m2) - l2, b2 = b ln 2.
 struct LpCoef {
-  float base, logs, c0, b, a;
+  float m2, l2, c0, b2, a;
   int64_t t;
+  // the second term. A masked logit (l = -inf) has p = 0: l is kept at -200, whose power is 0 too. A row of
+  // NaN statistics has a NaN c0.
+  __device__ __forceinline__ float others(float x) const {
+    const float l = fmaxf(fmaf(x, LOG2E, -m2) - l2, -200.f);
+    return -fast_exp2(l) * fmaf(b2, l, c0);
+  }
 };
 __device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* stats, const float* entropy,
                                           const float* dlogprobs, const float* dentropy, int64_t r, int V) {
   LpCoef c;
   c.t = tokens[r];
-  c.base = stats[2 * r];
-  c.logs = stats[2 * r + 1];
+  const float m = stats[2 * r], logs = stats[2 * r + 1];  // log p = (x - m) - logs
+  c.m2 = __fmul_rn(m, LOG2E);
+  c.l2 = logs * LOG2E - fmaf(-m, LOG2E, c.m2);
   c.a = c.t == -1 || !dlogprobs ? 0.f : dlogprobs[r];
   if (c.t < -1 || c.t >= V) c.a = __uint_as_float(0x7FC00000u);
-  c.b = dentropy ? dentropy[r] : 0.f;
-  c.c0 = c.a + (c.b != 0.f ? c.b * entropy[r] : 0.f);
+  const float b = dentropy ? dentropy[r] : 0.f;
+  c.b2 = b * LN2;
+  c.c0 = c.a + (b != 0.f ? b * entropy[r] : 0.f);
+  if (!(c.l2 < INFINITY && c.l2 > -INFINITY)) c.c0 = __uint_as_float(0x7FC00000u);
   return c;
 }
 
@@ -449,10 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             const int col0 = col_base + i * CW + hh * 32;
             tmem_ld_32x32(taddr + (uint32_t)(i * CW + hh * 32), v);
 #pragma unroll
-            for (int q = 0; q < 32; ++q) {
-              const float logp = (v[q] - c.base) - c.logs;
-              v[q] = -fast_exp2(logp * LOG2E) * fmaf(c.b, logp, c.c0);
-            }
+            for (int q = 0; q < 32; ++q) v[q] = c.others(v[q]);
             if (tok >= col0 && tok < col0 + 32) {
 #pragma unroll
               for (int q = 0; q < 32; ++q)
