@@ -34,8 +34,10 @@ def plain(x, tokens, k=0):
     ok = (tokens >= 0) & (tokens < V)
     lp = logp.gather(-1, torch.where(ok, tokens, 0)[..., None])[..., 0]
     lp = torch.where(ok, lp, torch.where(tokens == -1, 0.0, math.nan).double())
-    key = torch.where(x.isnan(), math.inf, x)  # stable: equal logits in id order
-    ids = torch.sort(key + 0.0, dim=-1, descending=True, stable=True).indices[..., :k]
+    # stable sorts: equal logits in id order, then NaN above all, +inf too
+    ids = torch.sort(torch.where(x.isnan(), math.inf, x) + 0.0, dim=-1, descending=True, stable=True).indices
+    nan = torch.sort(x.isnan().gather(-1, ids).int(), dim=-1, descending=True, stable=True).indices
+    ids = ids.gather(-1, nan)[..., :k]
     return lp, ent, ids, logp
 
 
@@ -217,6 +219,24 @@ def test_masked_backward():
     d, = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), x)
     assert bool((d[0, 10:] == 0).all()) and bool(d[0].isfinite().all()) and bool(d[3].isfinite().all())
     assert bool(d[1].isnan().all()) and bool(d[2].isnan().all())
+
+
+def test_rows_at_the_ends_of_the_range():
+    """Rows that hold nothing but the type's lowest value, or logits near its largest: values and
+    gradients as of any other row."""
+    big = 3e38
+    x = torch.full((5, 300), torch.finfo(torch.float32).min)
+    x[1, 7], x[1, 8] = big, big
+    x[2] = torch.linspace(-big, big, 300)  # (its step overflows: a row with NaN and +inf)
+    x[3] = 1e35 + torch.arange(300) * 0.0
+    x[4] = torch.linspace(-1, 1, 300) * big
+    x = x.cuda().requires_grad_()
+    t = torch.tensor([5, 7, 299, 0, 299]).cuda()
+    r = token_logprobs(x, t, top_k=2)
+    lp, ent, logp, rs = check_stats(r, x.detach(), t, 2)
+    a, b = torch.ones(5).cuda(), torch.full((5,), 0.5).cuda()
+    d, = torch.autograd.grad([r.logprobs, r.entropy], x, [a, b])
+    assert_close(d, plain_dx(logp, ent, t, a, b), 20 * rs + 1e-37)
 
 
 # ---- from hidden states -------------------------------------------------------------------------------

@@ -62,11 +62,30 @@ __device__ __forceinline__ float lp_add(LpStat& st, const float (&x)[NV]) {
     return st.s == st.s ? hi : INFINITY;
   }
   float s1 = 0.f, u1 = 0.f;
+  if (NV % 2 == 0) {
+    const uint64_t scale = f32x2(LOG2E, LOG2E), shift = f32x2(-st.m2, -st.m2);
+    uint64_t ss = 0, uu = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const float d = fmaf(x[i], LOG2E, -st.m2), e = fast_exp2(d);
-    s1 += e;
-    u1 = fmaf(e, d, u1);
+    for (int i = 0; i + 1 < NV; i += 2) {
+      const uint64_t d = f32x2_fma(f32x2(x[i], x[i + 1]), scale, shift);
+      float d0, d1;
+      f32x2_split(d, d0, d1);
+      const uint64_t e = f32x2(fast_exp2(d0), fast_exp2(d1));
+      ss = f32x2_add(ss, e);
+      uu = f32x2_fma(e, d, uu);
+    }
+    float s2, u2;
+    f32x2_split(ss, s1, s2);
+    f32x2_split(uu, u1, u2);
+    s1 += s2;
+    u1 += u2;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float d = fmaf(x[i], LOG2E, -st.m2), e = fast_exp2(d);
+      s1 += e;
+      u1 = fmaf(e, d, u1);
+    }
   }
   st.s += s1;
   st.u += u1;
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   __shared__ float2 wsum[LP_THREADS / 32];
   __shared__ alignas(16) LpStat runs[LP_MAX_SPLIT];                    // of the cluster's CTAs (first CTA)
   __shared__ uint64_t best[LP_MAX_SPLIT * LP_MAX_TOP];     // their alternatives, 0 for none (first CTA)
-  __shared__ float gmax[LP_GROUPS];
+  __shared__ alignas(16) float gmax[LP_GROUPS];
   __shared__ float kept[LP_KEPT * LP_THREADS];
   __shared__ float thr_s;
   __shared__ uint64_t cand[LP_CAP];
@@ -299,8 +318,12 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
     if (tid < LP_GROUPS) {
       int place = 0;
       const float mine = gmax[tid];
-#pragma unroll 8
-      for (int j = 0; j < LP_GROUPS; ++j) place += (gmax[j] > mine || (gmax[j] == mine && j < tid)) ? 1 : 0;
+#pragma unroll
+      for (int j = 0; j < LP_GROUPS; j += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(gmax + j);
+        place += (g.x > mine || (g.x == mine && j < tid)) + (g.y > mine || (g.y == mine && j + 1 < tid)) +
+                 (g.z > mine || (g.z == mine && j + 2 < tid)) + (g.w > mine || (g.w == mine && j + 3 < tid));
+      }
       if (place == k - 1) thr_s = mine;
     }
     __syncthreads();
@@ -327,6 +350,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
       for (int c = tid; c < n; c += LP_THREADS) {
         const uint64_t key = cand[c];
         int place = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) place += cand[j] > key ? 1 : 0;
         if (place < k) give(place, key);
       }
@@ -355,10 +379,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   if (rank != 0) return;
   LpStat all = runs[0];
   for (int i = 1; i < split; ++i) all = lp_merge(all, runs[i]);
-  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e. A row below -1e30 throughout has its
-  // statistics about -1e30 empty: those of a maximum of its own are taken in a second look.
+  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e. A row below -1e30 throughout leaves the sum
+  // about -1e30 empty, and one of 1e38 and more may have no m2: their sums are taken anew about the maximum.
   float base = all.m, logs = logf(all.s) + fmaf(-all.m, LOG2E, all.m2) * LN2, ent = logf(all.s) - LN2 * (all.u / all.s);
-  if (all.s == 0.f) {
+  if (all.s == 0.f || (all.m >= 1e38f && all.m < INFINITY)) {
     float hi = -INFINITY;
     for (int c = tid; c < V; c += LP_THREADS) hi = fmaxf(hi, lp_load(row + c));
     const float top = lp_key_value(lp_block_max(lp_key(hi, 0), red));
@@ -447,7 +471,7 @@ __global__ void __launch_bounds__(LP_THREADS)
     float v[NV];
     LpVec<T>::unpack(q, v);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = c.others(v[j]);
+    for (int j = 0; j < NV; j += 2) c.others2(v[j], v[j + 1]);
     dv[i] = LpVec<T>::pack(v);
   };
   int i = tid;
@@ -581,6 +605,36 @@ int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
   return std::min(N, cdiv(cdiv(N, cdiv(N, fit)), 256) * 256);
 }
 
+// Ranges of k into which the product (rows x D) over k of the backward is split.
+//
+// The tensor cores cut off what an accumulator cannot hold, a little with each step of 16 in k, always
+// towards zero: fp32 products are taken over ranges of about 512, as far as `room` floats hold their sums,
+// which are added with rounding (at 1001 x 4099 x 288 the gradients' error falls from 8e-6 to 1e-6).
+//
+// A bf16 product whose 256 x 256 tiles fill the CTA pairs badly (8192 x 768: 96 tiles, two rounds of 74) is
+// split where the rounds saved are worth writing and adding the partial sums (that one over 32000: 346 us,
+// split in three 260 + 15).
+int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
+  int splits = 1;
+  if (f32) {
+    splits = (int)std::min<int64_t>(room / (rows * D), cdiv(k, 512));
+  } else {
+    const int pairs = lp_sms() / 2;
+    const int64_t tiles = cdiv(rows, 256) * cdiv(D, 256);
+    const double round_us = 2.0 * 256 * 256 * (double)k / 19e6;   // of all pairs, at 1400 TFLOP/s
+    const double part_us = (double)rows * (double)D * 8 / 6.5e6;  // a partial sum, written and read
+    double least = (double)cdiv(tiles, pairs) * round_us;
+    for (int c = 2; c <= LP_MAX_K_SPLITS && c * 4096 <= k; ++c) {
+      const double t = (double)cdiv(tiles * c, pairs) / c * round_us + c * part_us + 5.0;
+      if (t < least) {
+        least = t;
+        splits = c;
+      }
+    }
+  }
+  return splits > 1 ? (int)cdiv(k, ksplit_chunk((int)k, splits)) : 1;  // no empty range
+}
+
 // The work buffer of the head's entries.
 struct LpWork {
   void *h_parts, *w_parts, *dx, *dx_parts;
@@ -606,8 +660,8 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     w.dx = take(N * ldv * (f32 ? 4 : 2));
     if (f32)
       w.dx_parts = take(3 * N * ldv * 2);
-    else  // partial sums of dh or dW, whichever is split
-      w.sums = floats(LP_MAX_K_SPLITS * std::max(N, V) * D);
+    else  // partial sums of dh, then of dW
+      w.sums = floats(std::max(lp_splits(N, V, D, false, 0) * N, lp_splits(V, N, D, false, 0) * V) * D);
   } else {
     const int64_t rows = lp_rows_at_once(N, V, k);
     // the shares of the rows of one launch: all of them, but for the last one's fewer rows
@@ -774,35 +828,13 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
     ww = w.w_parts;
     ld_h = ld_w = ldd;
   }
-  // Each product's operands are single matrices, or the three parts of one (its batches). The tensor cores
-  // cut off what an accumulator cannot hold, a little with each step of 16 in k, always towards zero: fp32
-  // products are taken over ranges of about 512, whose sums are added with rounding (at 1001 x 4099 x 288
-  // the gradients' error falls from 8e-6 to below 2e-6). The ranges' sums take the place of the fp32
-  // gradient of the logits, which its parts have replaced.
-  //
-  // A bf16 product whose 256 x 256 tiles fill the CTA pairs badly (8192 x 768: 96 tiles, two rounds of 74)
-  // is split over k too, where the rounds saved are worth writing and adding the partial sums.
-  const int pairs = lp_sms() / 2;
+  // Each product's operands are single matrices, or the three parts of one (its batches); its partial sums
+  // (lp_splits) of fp32 operands take the place of the fp32 gradient of the logits, which its parts have
+  // replaced.
   auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) -> int {
     GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
     g.parts = f32 ? 6 : 0;
-    int splits = 1;
-    if (f32) {
-      splits = (int)std::min<int64_t>(N * ldv / (rows * D), cdiv(k, 512));
-    } else {
-      const int64_t tiles = cdiv(rows, 256) * cdiv(D, 256);
-      const double round_us = 2.0 * 256 * 256 * (double)k / 19e6;   // of all pairs, at 1400 TFLOP/s
-      const double part_us = (double)rows * (double)D * 8 / 6.5e6;  // a partial sum, written and read
-      double least = (double)cdiv(tiles, pairs) * round_us;
-      for (int c = 2; c <= LP_MAX_K_SPLITS && c * 4096 <= k; ++c) {
-        const double t = (double)cdiv(tiles * c, pairs) / c * round_us + c * part_us + 5.0;
-        if (t < least) {
-          least = t;
-          splits = c;
-        }
-      }
-    }
-    if (splits > 1) splits = (int)cdiv(k, ksplit_chunk((int)k, splits));
+    const int splits = lp_splits(rows, k, D, f32, f32 ? N * ldv : 0);
     if (splits <= 1) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
     g.batches = g.ksplit = splits;
     float* sums = f32 ? static_cast<float*>(w.dx) : w.sums;

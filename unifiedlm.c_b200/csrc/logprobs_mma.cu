@@ -98,25 +98,32 @@ struct LpArgs {
   const float* dentropy;
 };
 
-// The backward's factors of one row: dx_v = [v = t] a - p_v (a + b (log p_v + H)), in base 2 as the
-// statistics are: p_v = 2^l, l = (x_v log2 e - m2) - l2, b2 = b ln 2.
+// The backward's factors of one row: dx_v = [v = t] a - p_v (a + b (log p_v + H)), with p_v = 2^l,
+// l = (x_v - m) log2 e - l2, b2 = b ln 2.
 struct LpCoef {
-  float m2, l2, c0, b2, a;
+  float m, l2, c0, b2, a;
   int64_t t;
   // the second term. A masked logit (l = -inf) has p = 0: l is kept at -200, whose power is 0 too. A row of
   // NaN statistics has a NaN c0.
   __device__ __forceinline__ float others(float x) const {
-    const float l = fmaxf(fmaf(x, LOG2E, -m2) - l2, -200.f);
+    const float l = fmaxf(fmaf(x - m, LOG2E, -l2), -200.f);
     return -fast_exp2(l) * fmaf(b2, l, c0);
+  }
+  __device__ __forceinline__ void others2(float& x, float& y) const {
+    float lx, ly;
+    f32x2_split(f32x2_fma(f32x2_add(f32x2(x, y), f32x2(-m, -m)), f32x2(LOG2E, LOG2E), f32x2(-l2, -l2)), lx, ly);
+    lx = fmaxf(lx, -200.f);
+    ly = fmaxf(ly, -200.f);
+    const uint64_t q = f32x2_fma(f32x2(-b2, -b2), f32x2(lx, ly), f32x2(-c0, -c0));
+    f32x2_split(f32x2_mul(f32x2(fast_exp2(lx), fast_exp2(ly)), q), x, y);
   }
 };
 __device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* stats, const float* entropy,
                                           const float* dlogprobs, const float* dentropy, int64_t r, int V) {
   LpCoef c;
   c.t = tokens[r];
-  const float m = stats[2 * r], logs = stats[2 * r + 1];  // log p = (x - m) - logs
-  c.m2 = __fmul_rn(m, LOG2E);
-  c.l2 = logs * LOG2E - fmaf(-m, LOG2E, c.m2);
+  c.m = stats[2 * r];
+  c.l2 = stats[2 * r + 1] * LOG2E;
   c.a = c.t == -1 || !dlogprobs ? 0.f : dlogprobs[r];
   if (c.t < -1 || c.t >= V) c.a = __uint_as_float(0x7FC00000u);
   const float b = dentropy ? dentropy[r] : 0.f;
@@ -187,16 +194,20 @@ struct LpRun {
       m = lm;
       m2 = n2;
     }
-    float s0 = 0.f, s1 = 0.f, u0 = 0.f, u1 = 0.f;
+    const uint64_t scale = f32x2(LOG2E, LOG2E), shift = f32x2(-m2, -m2);
+    uint64_t ss[2] = {0, 0}, uu[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-      const float d0 = fmaf(x[i], LOG2E, -m2), d1 = fmaf(x[i + 1], LOG2E, -m2);
-      const float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
-      s0 += e0;
-      s1 += e1;
-      u0 = fmaf(e0, d0, u0);
-      u1 = fmaf(e1, d1, u1);
+      const uint64_t d = f32x2_fma(f32x2(x[i], x[i + 1]), scale, shift);
+      float d0, d1;
+      f32x2_split(d, d0, d1);
+      const uint64_t e = f32x2(fast_exp2(d0), fast_exp2(d1));
+      ss[i / 2 % 2] = f32x2_add(ss[i / 2 % 2], e);
+      uu[i / 2 % 2] = f32x2_fma(e, d, uu[i / 2 % 2]);
     }
+    float s0, s1, u0, u1;
+    f32x2_split(f32x2_add(ss[0], ss[1]), s0, s1);
+    f32x2_split(f32x2_add(uu[0], uu[1]), u0, u1);
     s += s0 + s1;
     u += u0 + u1;
   }
@@ -459,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             const int col0 = col_base + i * CW + hh * 32;
             tmem_ld_32x32(taddr + (uint32_t)(i * CW + hh * 32), v);
 #pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = c.others(v[q]);
+            for (int q = 0; q < 32; q += 2) c.others2(v[q], v[q + 1]);
             if (tok >= col0 && tok < col0 + 32) {
 #pragma unroll
               for (int q = 0; q < 32; ++q)
