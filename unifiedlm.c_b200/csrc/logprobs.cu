@@ -819,10 +819,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
     return rc;
   const void *dx = w.dx, *hh = h_op, *ww = w_op;
   if (f32) {
-    const int64_t ctas = cdiv(N * ldv, 256 * 8);
-    if (int rc = launch_pdl(lp_split_kernel, dim3((unsigned)(ctas < 8192 ? ctas : 8192)), dim3(256), 0, st,
-                            static_cast<const float*>(w.dx), ldv, static_cast<__nv_bfloat16*>(w.dx_parts), ldv, N, V))
-      return rc;
+    if (int rc = lp_split(static_cast<const float*>(w.dx), ldv, w.dx_parts, ldv, N, V, st)) return rc;
     dx = w.dx_parts;
     hh = w.h_parts;
     ww = w.w_parts;

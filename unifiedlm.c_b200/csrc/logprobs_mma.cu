@@ -764,25 +764,37 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
 }
 constexpr int LP_MAX_GROUPS = 128;
 
-// hi, mid and lo of fp32 rows (n, d), ld apart, as three bf16 matrices of row stride ld_o
+// hi, mid and lo of fp32 rows (n, d), ld apart, as three bf16 matrices of row stride ld_o (a multiple of 8,
+// the rest zero); a thread takes two neighbours
 __global__ void __launch_bounds__(256)
     lp_split_kernel(const float* __restrict__ x, int64_t ld, __nv_bfloat16* __restrict__ out, int64_t ld_o, int64_t rows,
                     int64_t d) {
   pdl_enter();
-  const int64_t n = rows * ld_o;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / ld_o, c = i - r * ld_o;
-    const float v = c < d ? x[r * ld + c] : 0.f;
-    __nv_bfloat16 hi = __float2bfloat16_rn(v);
+  const int64_t part = rows * ld_o / 2;  // pairs of one matrix
+  uint32_t* o = reinterpret_cast<uint32_t*>(out);
+  auto split = [](float v, __nv_bfloat16& hi, __nv_bfloat16& mid, __nv_bfloat16& lo) {
+    hi = __float2bfloat16_rn(v);
     if (isinf(__bfloat162float(hi)) && !isinf(v)) hi = __float2bfloat16_rz(v);
-    const float fh = __bfloat162float(hi);
-    const float rest = isfinite(v) ? v - fh : 0.f;
-    const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
-    const __nv_bfloat16 lo = __float2bfloat16_rn(rest - __bfloat162float(mid));
-    out[i] = hi;
-    out[n + i] = mid;
-    out[2 * n + i] = lo;
+    const float rest = isfinite(v) ? v - __bfloat162float(hi) : 0.f;
+    mid = __float2bfloat16_rn(rest);
+    lo = __float2bfloat16_rn(rest - __bfloat162float(mid));
+  };
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float* row = x + r * ld;
+#pragma unroll 4
+    for (int64_t c = threadIdx.x; c < ld_o / 2; c += 256) {
+      __nv_bfloat162 p[3];
+      split(2 * c < d ? row[2 * c] : 0.f, p[0].x, p[1].x, p[2].x);
+      split(2 * c + 1 < d ? row[2 * c + 1] : 0.f, p[0].y, p[1].y, p[2].y);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) o[i * part + r * (ld_o / 2) + c] = *reinterpret_cast<const uint32_t*>(&p[i]);
+    }
   }
+}
+
+int lp_split(const float* x, int64_t ld, void* out, int64_t ld_o, int64_t rows, int64_t d, cudaStream_t st) {
+  return launch_pdl(lp_split_kernel, dim3((unsigned)std::min<int64_t>(rows, 1 << 20)), dim3(256), 0, st, x, ld,
+                    static_cast<__nv_bfloat16*>(out), ld_o, rows, d);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------
@@ -831,10 +843,7 @@ int lp_operand(CUtensorMap* map, const void* x, int64_t ld, int64_t rows, int64_
                cudaStream_t st) {
   if (f32) {
     const int64_t ld_o = ulm_operand_ld(D);
-    const int64_t ctas = cdiv(rows * ld_o, 256 * 8);
-    if (int rc = launch_pdl(lp_split_kernel, dim3((unsigned)(ctas < 8192 ? ctas : 8192)), dim3(256), 0, st,
-                            static_cast<const float*>(x), ld, static_cast<__nv_bfloat16*>(parts), ld_o, rows, D))
-      return rc;
+    if (int rc = lp_split(static_cast<const float*>(x), ld, parts, ld_o, rows, D, st)) return rc;
     return make_tmap(map, Operand{parts, ld_o, rows * ld_o, D, rows, ULM_BF16, false}, 3, 64, 128);
   }
   ULM_REQUIRE(is_aligned16(x) && ld % 8 == 0, "bf16 operands must be 16-byte aligned, their row stride a multiple of 8");
