@@ -461,13 +461,13 @@ int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const 
                            int64_t N, int64_t V, void* stream);
 
 /* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd.
- * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 256-byte aligned. */
+ * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 16-byte aligned. */
 int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens,
                              float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
                              void* work, int64_t N, int64_t V, int64_t D, int top_k, int prec, void* stream);
 /* Backward: dh (N,D) of dh_dtype and dw (V,D) of dw_dtype (either may be NULL: not wanted); the logits
  * are recomputed. work:
- * ulm_lm_head_logprobs_work_bytes(N,V,D,0,1,prec) bytes, 256-byte aligned. */
+ * ulm_lm_head_logprobs_work_bytes(N,V,D,0,1,prec) bytes, 16-byte aligned. */
 int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* dentropy, const void* h_op, int64_t ld_h,
                              const void* w_op, int64_t ld_w, const int64_t* tokens, const float* stats,
                              const float* entropy, void* dh, int dh_dtype, void* dw, int dw_dtype, void* work,
@@ -482,7 +482,7 @@ int ulm_embedding_fwd(const int64_t* tokens, const void* weight, int w_dtype, in
                       int64_t N, int64_t V, int64_t D, float scale, void* stream);
 /* Backward: dw (V,D) of dw_dtype (overwritten) = scale * the sum of dy's rows (N,D) of dy_dtype by
  * token, in fp32 and in a fixed order; tokens outside [0,V) add nothing. work:
- * ulm_embedding_bwd_work_bytes(N,V,D) bytes. */
+ * ulm_embedding_bwd_work_bytes(N,V,D) bytes, 16-byte aligned. */
 int ulm_embedding_bwd(const int64_t* tokens, const void* dy, int dy_dtype, void* dw, int dw_dtype, void* work,
                       int64_t N, int64_t V, int64_t D, float scale, void* stream);
 int64_t ulm_embedding_bwd_work_bytes(int64_t N, int64_t V, int64_t D);

@@ -60,6 +60,7 @@ def test_head_logprobs_arguments():
     refused(fwd(ld_h=15), "stride")
     refused(fwd(ld_w=15), "stride")
     refused(fwd(work=None), "null")
+    refused(fwd(work=ctypes.c_void_p(264)), "aligned")
     refused(fwd(h=None), "null")
     refused(fwd(D=0), "extent")
     refused(fwd(k=9), "top_k")
@@ -90,6 +91,7 @@ def test_embedding_arguments():
     refused(lib.ulm_embedding_bwd(P, P, 4, P, 0, P, 2, 4, 8, 1.0, None), "dtype")
     refused(lib.ulm_embedding_bwd(P, P, 0, None, 0, P, 2, 4, 8, 1.0, None), "null")
     refused(lib.ulm_embedding_bwd(P, P, 0, P, 0, None, 2, 4, 8, 1.0, None), "null")
+    refused(lib.ulm_embedding_bwd(P, P, 0, P, 0, ctypes.c_void_p(264), 2, 4, 8, 1.0, None), "aligned")
     assert lib.ulm_embedding_bwd_work_bytes(1, -1, 8) == -1
 
 
@@ -111,6 +113,7 @@ def test_clip_arguments():
     refused(call([4096], [4096], counts=[-1]), "count")
     refused(call([4096], [4096], norm=None), "null")
     refused(call([4096], [4096], work=None), "null")
+    refused(call([4096], [4096], work=ctypes.c_void_p(260)), "aligned")
     refused(call([4096, 4096], [4096, 4096]), "overlap")           # the same tensor twice
     refused(call([4096, 4100], [4096, 4100]), "overlap")           # a view of another one
     refused(call([4096, 8192], [8192, 4096]), "overlap")           # swapped

@@ -265,6 +265,7 @@ static int clip_grads_impl(const void* const* grads, void* const* outs, const in
   ULM_REQUIRE(n >= 0 && n < (1 << 24), "bad number of tensors %lld", (long long)n);
   ULM_REQUIRE(norm && work && (n == 0 || (grads && counts && in_dtypes)), "null pointer argument");
   ULM_REQUIRE(!outs || n == 0 || out_dtypes, "null pointer argument");
+  ULM_REQUIRE((reinterpret_cast<uintptr_t>(work) & 7) == 0, "work must be 8-byte aligned");
   ULM_REQUIRE(!outs || max_norm >= 0.f, "max_norm must not be negative or NaN");
   for (int64_t i = 0; i < n; ++i) {
     ULM_REQUIRE(counts[i] >= 0 && counts[i] < (1ll << 42), "bad element count of tensor %lld", (long long)i);

@@ -742,6 +742,7 @@ extern "C" int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const vo
   if (int rc = lp_check_top(N, V, top_k, top_ids, top_logprobs)) return rc;
   if (N == 0) return ULM_OK;
   ULM_REQUIRE(logprobs && entropy && work, "null pointer argument");
+  ULM_REQUIRE(is_aligned16(work), "work must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f32 = prec == ULM_PREC_FP32;
   const LpWork w = lp_work(work, N, V, D, top_k, false, f32);
@@ -794,6 +795,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   if (int rc = lp_head_check(h_op, ld_h, w_op, ld_w, tokens, N, V, D, prec)) return rc;
   ULM_REQUIRE(lp_dtype_ok(dh_dtype) && lp_dtype_ok(dw_dtype), "bad dtype");
   ULM_REQUIRE(N == 0 || (stats && entropy && work), "null pointer argument");
+  ULM_REQUIRE(N == 0 || is_aligned16(work), "work must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!dh && !dw) return ULM_OK;
   if (N == 0) {
