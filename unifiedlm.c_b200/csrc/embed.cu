@@ -130,6 +130,7 @@ constexpr int SORT_CTAS = 8;  // one cluster
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int SORT_BINS = 256;
+constexpr int SORT_AHEAD = 4;  // entries of a lane loaded before the first is used
 constexpr int EMB_FILL_CTAS = 288;  // with the sort's, two CTAs of 1024 threads on each SM
 
 // A shared-memory word of CTA `rank` of the cluster
@@ -151,12 +152,26 @@ __device__ __forceinline__ void emb_fill(char* p, int64_t bytes, int64_t i, int6
   for (int64_t b = tail + 2 * i; b < bytes; b += 2 * n) *reinterpret_cast<uint16_t*>(p + b) = 0;
 }
 
+// The lanes of the warp that hold the same digit, of those with one (Nine votes: match.any took 8700 cycles
+// where they take 5600.)
+__device__ __forceinline__ uint32_t sort_same(int digit, bool has) {
+  uint32_t same = __ballot_sync(0xffffffffu, has);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const bool bit = (digit >> b) & 1;
+    const uint32_t set = __ballot_sync(0xffffffffu, bit);
+    same &= bit ? set : ~set;
+  }
+  return same;
+}
+
 // CTAs 0 .. 7: the sorted (key, position) pairs, keys the tokens, or V for what is none (these come last).
 // Each warp owns a run of consecutive entries. A pass counts digits by warp, turns the counts into the
-// warps' first places (over the warps, the CTAs, and the digits), and moves the entries in order. `key`
-// and `pos` hold two buffers of N each; pass p writes buffer p % 2. All other CTAs zero dW.
+// warps' first places (over the warps, the CTAs, and the digits), and moves the entries in order, key and
+// position in one 8-byte store (the scattered stores bound a pass: 32 sectors a warp). `sorted` holds two
+// buffers of N; pass p writes buffer p % 2. All other CTAs zero dW.
 __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
-    embed_sort_kernel(const int64_t* __restrict__ tokens, int* __restrict__ key, int* __restrict__ pos, int N, int V,
+    embed_sort_kernel(const int64_t* __restrict__ tokens, int2* __restrict__ sorted, int N, int V,
                       int passes, char* __restrict__ dw, int64_t dw_bytes) {
   __shared__ uint32_t cnt[SORT_WARPS][SORT_BINS];
   __shared__ uint32_t total[SORT_BINS], base[SORT_BINS], wsum[SORT_BINS / 32];
@@ -171,25 +186,28 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
   const int64_t own = ((int64_t)N + SORT_CTAS * SORT_WARPS * 32 - 1) / (SORT_CTAS * SORT_WARPS * 32) * 32;
   const int64_t i0 = ((int64_t)rank * SORT_WARPS + w) * own, i1 = min((int64_t)N, i0 + own);
   for (int p = 0; p < passes; ++p) {
-    const int* ksrc = key + (int64_t)((p + 1) & 1) * N;
-    const int* psrc = pos + (int64_t)((p + 1) & 1) * N;
-    int* kdst = key + (int64_t)(p & 1) * N;
-    int* pdst = pos + (int64_t)(p & 1) * N;
-    auto load_key = [&](int64_t i) -> int {
-      if (i >= i1) return -1;
-      if (p > 0) return __ldcg(ksrc + i);
+    const int2* src = sorted + (int64_t)((p + 1) & 1) * N;
+    int2* dst = sorted + (int64_t)(p & 1) * N;
+    auto load = [&](int64_t i) -> int2 {
+      if (i >= i1) return make_int2(-1, 0);
+      if (p > 0) return __ldcg(src + i);
       const int64_t t = tokens[i];
-      return t >= 0 && t < V ? (int)t : V;
+      return make_int2(t >= 0 && t < V ? (int)t : V, (int)i);
     };
     for (int b = lane; b < SORT_BINS; b += 32) cnt[w][b] = 0;
     __syncwarp();
-#pragma unroll 4
-    for (int64_t i = i0; i < i1; i += 32) {
-      const int k = load_key(i + lane);
-      const int d = k < 0 ? SORT_BINS : (k >> (8 * p)) & (SORT_BINS - 1);
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (k >= 0 && lane == __ffs(same) - 1) cnt[w][d] += __popc(same);
-      __syncwarp();
+    for (int64_t i = i0; i < i1; i += 32 * SORT_AHEAD) {
+      int k[SORT_AHEAD];
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) k[j] = load(i + 32 * j + lane).x;
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) {
+        if (i + 32 * j >= i1) break;
+        const int d = (k[j] >> (8 * p)) & (SORT_BINS - 1);
+        const uint32_t same = sort_same(d, k[j] >= 0);
+        if (k[j] >= 0 && lane == __ffs(same) - 1) cnt[w][d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (tid < SORT_BINS) {
@@ -226,21 +244,24 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
       base[tid] = off + incl - all + before;
     }
     __syncthreads();
-#pragma unroll 2
-    for (int64_t i = i0; i < i1; i += 32) {
-      const int k = load_key(i + lane);
-      const int at = k < 0 ? 0 : p > 0 ? __ldcg(psrc + i + lane) : (int)(i + lane);
-      const int d = k < 0 ? SORT_BINS : (k >> (8 * p)) & (SORT_BINS - 1);
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      uint32_t to = 0;
-      if (k >= 0) to = base[d] + cnt[w][d] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (k >= 0) {
-        if (lane == __ffs(same) - 1) cnt[w][d] += __popc(same);
-        kdst[to] = k;
-        pdst[to] = at;
+    for (int64_t i = i0; i < i1; i += 32 * SORT_AHEAD) {
+      int2 e[SORT_AHEAD];
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) e[j] = load(i + 32 * j + lane);
+#pragma unroll
+      for (int j = 0; j < SORT_AHEAD; ++j) {
+        if (i + 32 * j >= i1) break;
+        const int d = (e[j].x >> (8 * p)) & (SORT_BINS - 1);
+        const uint32_t same = sort_same(d, e[j].x >= 0);
+        uint32_t to = 0;
+        if (e[j].x >= 0) to = base[d] + cnt[w][d] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (e[j].x >= 0) {
+          if (lane == __ffs(same) - 1) cnt[w][d] += __popc(same);
+          dst[to] = e[j];
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     // the places of this pass are read by the whole cluster in the next one
     cluster_sync_all();
@@ -256,7 +277,7 @@ constexpr int EMB_CHUNK = 32;  // sorted entries of one warp
 // of a run that begins in it and goes on.
 template <typename E, int NV>
 __global__ void __launch_bounds__(EMB_THREADS)
-    embed_sum_kernel(const int* __restrict__ key, const int* __restrict__ pos, const E* __restrict__ dy,
+    embed_sum_kernel(const int2* __restrict__ sorted, const E* __restrict__ dy,
                      void* __restrict__ dw, int dw_dtype, float* __restrict__ part, int N, int V, int64_t D,
                      int col_blocks, float scale) {
   pdl_enter();
@@ -268,10 +289,10 @@ __global__ void __launch_bounds__(EMB_THREADS)
   const int64_t d = (item - c * col_blocks) * (32 * NV) + lane * NV;
   const bool in = d < D;
   const int n = (int)min((int64_t)EMB_CHUNK, N - i0);
-  const int k = lane < n ? key[i0 + lane] : V;
-  const int p = lane < n ? pos[i0 + lane] : 0;
-  const int next_chunk = i0 + EMB_CHUNK < N ? key[i0 + EMB_CHUNK] : V;
-  const int last_chunk = i0 > 0 ? key[i0 - 1] : -1;
+  const int2 mine = lane < n ? sorted[i0 + lane] : make_int2(V, 0);
+  const int k = mine.x, p = mine.y;
+  const int next_chunk = i0 + EMB_CHUNK < N ? sorted[i0 + EMB_CHUNK].x : V;
+  const int last_chunk = i0 > 0 ? sorted[i0 - 1].x : -1;
   int next = __shfl_down_sync(0xffffffffu, k, 1);
   if (lane == EMB_CHUNK - 1) next = next_chunk;
   const uint32_t ends = __ballot_sync(0xffffffffu, k != next);  // entries that end their run
@@ -282,34 +303,33 @@ __global__ void __launch_bounds__(EMB_THREADS)
   for (int i = 0; i < NV; ++i) acc[i] = 0.f;
   bool first = cont;  // the run at hand began before this chunk
   const int m = __popc(live);  // the entries of tokens: they come first
-  constexpr int U = 8;
+  constexpr int U = 8;  // rows in flight
 #pragma unroll 1
   for (int j0 = 0; j0 < m; j0 += U) {
-    float x[U][NV];
+    uint4 q[U];  // 16 bytes, or one element in the first word
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = __shfl_sync(0xffffffffu, p, (j0 + u) & 31);
+      q[u] = make_uint4(0, 0, 0, 0);
       if (in && j0 + u < m) {
-        if (NV == 1) {
-          x[u][0] = sizeof(E) == 4 ? reinterpret_cast<const float*>(dy)[row * D + d]
-                                   : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(dy)[row * D + d]);
-        } else {
-          float t[EmbVec<E>::N];
-          EmbVec<E>::unpack(*reinterpret_cast<const uint4*>(dy + row * D + d), t);
-#pragma unroll
-          for (int i = 0; i < NV; ++i) x[u][i] = t[i % EmbVec<E>::N];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) x[u][i] = 0.f;
+        if (NV == 1)
+          q[u].x = __float_as_uint(emb_load(dy, sizeof(E) == 4 ? ULM_F32 : ULM_BF16, row * D + d));
+        else
+          q[u] = *reinterpret_cast<const uint4*>(dy + row * D + d);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u;
       if (j >= m) break;
+      if (NV == 1) {
+        acc[0] += __uint_as_float(q[u].x);
+      } else {
+        float x[EmbVec<E>::N];
+        EmbVec<E>::unpack(q[u], x);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) acc[i] += x[u][i];
+        for (int i = 0; i < NV; ++i) acc[i] += x[i % EmbVec<E>::N];
+      }
       const bool end = (ends >> j) & 1u;
       if (!end && j + 1 < EMB_CHUNK) continue;
       const int64_t v = __shfl_sync(0xffffffffu, k, j);
@@ -353,14 +373,15 @@ __global__ void __launch_bounds__(EMB_THREADS)
 // adds every eighth one, then the warps' sums are added in order.
 template <int NV>
 __global__ void __launch_bounds__(EMB_THREADS)
-    embed_join_kernel(const int* __restrict__ key, const float* __restrict__ part, void* __restrict__ dw, int dw_dtype,
+    embed_join_kernel(const int2* __restrict__ sorted, const float* __restrict__ part, void* __restrict__ dw, int dw_dtype,
                       int N, int V, int64_t D, float scale) {
   pdl_enter();
   __shared__ float red[EMB_THREADS / 32][32 * NV];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = blockIdx.x, i0 = c * EMB_CHUNK, last = i0 + EMB_CHUNK - 1;
   if (last + 1 >= N) return;
-  const int k = key[last], after = key[last + 1], begin = key[i0], before = i0 > 0 ? key[i0 - 1] : -1;
+  const int k = sorted[last].x, after = sorted[last + 1].x, begin = sorted[i0].x;
+  const int before = i0 > 0 ? sorted[i0 - 1].x : -1;
   if (k >= V || after != k) return;            // no run goes on
   if (begin == k && before == k) return;       // it began in an earlier chunk
   // chunks c + 1 .. c + more begin with entries of the same run
@@ -368,7 +389,7 @@ __global__ void __launch_bounds__(EMB_THREADS)
   int64_t more = 0;
   for (;;) {
     const int64_t cc = c + 1 + more + lane;
-    const uint32_t b = __ballot_sync(0xffffffffu, cc < chunks && key[cc * EMB_CHUNK] == k);
+    const uint32_t b = __ballot_sync(0xffffffffu, cc < chunks && sorted[cc * EMB_CHUNK].x == k);
     if (b == 0xffffffffu) {
       more += 32;
     } else {
@@ -416,8 +437,7 @@ int emb_check(const int64_t* tokens, int64_t N, int64_t V, int64_t D) {
 bool emb_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
 struct EmbWork {
-  int* key;
-  int* pos;
+  int2* sorted;
   float* part;
   int64_t bytes;
 };
@@ -425,15 +445,14 @@ EmbWork emb_work(void* base, int64_t N, int64_t D) {
   auto al = [](int64_t n) { return (n + 255) / 256 * 256; };
   char* p = static_cast<char*>(base);
   EmbWork w;
-  w.key = reinterpret_cast<int*>(p);
-  w.pos = reinterpret_cast<int*>(p + al(2 * N * 4));
-  w.part = reinterpret_cast<float*>(p + 2 * al(2 * N * 4));
-  w.bytes = 2 * al(2 * N * 4) + al(2 * cdiv(N, EMB_CHUNK) * D * 4);
+  w.sorted = reinterpret_cast<int2*>(p);
+  w.part = reinterpret_cast<float*>(p + al(2 * N * 8));
+  w.bytes = al(2 * N * 8) + al(2 * cdiv(N, EMB_CHUNK) * D * 4);
   return w;
 }
 
 template <typename E>
-int emb_sums(const EmbWork& w, const int* key, const int* pos, const void* dy, void* dw, int dw_dtype, int64_t N,
+int emb_sums(const EmbWork& w, const int2* sorted, const void* dy, void* dw, int dw_dtype, int64_t N,
              int64_t V, int64_t D, float scale, cudaStream_t st) {
   constexpr int NV = EmbVec<E>::N;
   const bool vec = D % 8 == 0 && is_aligned16(dy) && is_aligned16(dw);
@@ -441,12 +460,12 @@ int emb_sums(const EmbWork& w, const int* key, const int* pos, const void* dy, v
   const int64_t ctas = cdiv(chunks * cols, EMB_THREADS / 32);
   ULM_REQUIRE(ctas < (1ll << 31) && cdiv(D, 32) < 65536, "extent too large");
   auto kern = vec ? embed_sum_kernel<E, NV> : embed_sum_kernel<E, 1>;
-  if (int rc = launch_pdl(kern, dim3((unsigned)ctas), dim3(EMB_THREADS), 0, st, key, pos, static_cast<const E*>(dy), dw,
+  if (int rc = launch_pdl(kern, dim3((unsigned)ctas), dim3(EMB_THREADS), 0, st, sorted, static_cast<const E*>(dy), dw,
                           dw_dtype, w.part, (int)N, (int)V, D, (int)cols, scale))
     return rc;
   if (chunks < 2) return ULM_OK;
   return launch_pdl(vec ? embed_join_kernel<4> : embed_join_kernel<1>,
-                    dim3((unsigned)(chunks - 1), (unsigned)cdiv(D, vec ? 128 : 32)), dim3(EMB_THREADS), 0, st, key,
+                    dim3((unsigned)(chunks - 1), (unsigned)cdiv(D, vec ? 128 : 32)), dim3(EMB_THREADS), 0, st, sorted,
                     static_cast<const float*>(w.part), dw, dw_dtype, (int)N, (int)V, D, scale);
 }
 
@@ -500,10 +519,10 @@ extern "C" int ulm_embedding_bwd(const int64_t* tokens, const void* dy, int dy_d
   const EmbWork w = emb_work(work, N, D);
   int passes = 1;
   while (V >> (8 * passes)) ++passes;  // keys are 0 .. V
-  if (int rc = launch_pdl(embed_sort_kernel, dim3(SORT_CTAS + EMB_FILL_CTAS), dim3(SORT_THREADS), 0, st, tokens, w.key,
-                          w.pos, (int)N, (int)V, passes, static_cast<char*>(dw), dw_bytes))
+  if (int rc = launch_pdl(embed_sort_kernel, dim3(SORT_CTAS + EMB_FILL_CTAS), dim3(SORT_THREADS), 0, st, tokens,
+                          w.sorted, (int)N, (int)V, passes, static_cast<char*>(dw), dw_bytes))
     return rc;
   const int64_t last = (int64_t)((passes - 1) & 1) * N;
-  return dy_dtype == ULM_F32 ? emb_sums<float>(w, w.key + last, w.pos + last, dy, dw, dw_dtype, N, V, D, scale, st)
-                             : emb_sums<__nv_bfloat16>(w, w.key + last, w.pos + last, dy, dw, dw_dtype, N, V, D, scale, st);
+  return dy_dtype == ULM_F32 ? emb_sums<float>(w, w.sorted + last, dy, dw, dw_dtype, N, V, D, scale, st)
+                             : emb_sums<__nv_bfloat16>(w, w.sorted + last, dy, dw, dw_dtype, N, V, D, scale, st);
 }
