@@ -313,6 +313,27 @@ def test_head_backward(precision, dtype, N, V, D):
     assert L.device_error() == 0
 
 
+@pytest.mark.parametrize("N,V,D", [(1, 700, 64), (7, 9000, 288), (256, 3000, 96)])
+def test_head_backward_of_few_rows_rounds_once(N, V, D):
+    """bf16 operands, up to 256 rows: the logits' gradient goes into the products in two bf16 parts (16
+    digits), so that dh and dW are off by their own rounding alone: each value by half a step, and by the
+    fp32 sums and 2^-17 of the terms' magnitudes before it."""
+    h, w, t, gen = head_inputs(N, V, D, torch.bfloat16, N)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    a, b = torch.randn(N, generator=gen).cuda(), torch.randn(N, generator=gen).cuda()
+    r = lm_head_logprobs(h, w, t)
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [h, w], [a, b])
+    h64, w64 = h.detach().double(), w.detach().double()
+    lp, ent, _, logp = plain(h64 @ w64.t(), t)
+    d = plain_dx(logp, ent, t, a, b)
+    rs = tol_s(V, 20.0) + 2 * head_extra(h64, w64, D)
+    size = logp.exp() * (a.abs().double()[:, None] + b.abs().double()[:, None] * (logp.abs() + ent[:, None]))
+    d_err = size * 8 * rs + (d.abs() + size) * 2.0 ** -17
+    for got, want, err, mag, n in ((dh, d @ w64, d_err @ w64.abs(), d.abs() @ w64.abs(), V),
+                                   (dw, d.t() @ h64, d_err.t() @ h64.abs(), d.abs().t() @ h64.abs(), N)):
+        assert_close(got, want, err + (n / 16 + 16) * 4 * U * mag + HALF[torch.bfloat16] * want.abs() + 1e-30)
+
+
 def test_head_mixed_types_strides_and_empty():
     h = torch.randn(6, 4, 70, device="cuda")[..., :64].requires_grad_()  # rows of stride 70
     w = torch.randn(200, 64, device="cuda").bfloat16().requires_grad_()

@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
         const int n1 = kb1 - kb0;
-        const int nkb = shape.parts ? 6 * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         for (int i = 0; i < nkb; ++i) {
           if (!wait_or_abort(&empty[stage], phase ^ 1u, abort_flag, DEVERR_GEMM_PRODUCER_WAIT)) {
@@ -883,8 +883,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
           const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
-          const int oa = shape.parts ? GEMM_PART_A[part] : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = shape.parts ? GEMM_PART_B[part] : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int oa = shape.parts ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = shape.parts ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d(ma, sa, &full[stage], k0, tc.mb * TC_BM, oa);
           } else {
@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = shape.parts ? 6 * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1172,7 +1172,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
         const int n1 = kb1 - kb0;
-        const int nkb = shape.parts ? 6 * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         const int row0 = tc.mb * BM + (int)rank * 128;
         const int col0 = tc.nb * BN + (int)rank * 128;
@@ -1191,8 +1191,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
           const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
-          const int oa = shape.parts ? GEMM_PART_A[part] : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = shape.parts ? GEMM_PART_B[part] : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int oa = shape.parts ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = shape.parts ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d_pair(ma, sa, bar, k0, row0, oa);
           } else {
@@ -1268,7 +1268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = shape.parts ? 6 * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = shape.parts ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1674,10 +1674,11 @@ int launch_tc(const Operand& A, const Operand& B, const Operand* A2, const Opera
               const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = TcConfig<BN>;
   CUtensorMap ta, tb, ta2, tb2, tout, taux;
-  const int ob = s.parts ? 3 : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int ob = s.parts ? (s.parts == 6 ? 3 : 2) : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int obb = s.parts == 2 ? 1 : ob;
   int rc = make_tmap(&ta, A, ob, 64, A_MN ? 64 : TC_BM);
   if (rc) return rc;
-  rc = make_tmap(&tb, B, ob, 64, B_MN ? 64 : BN);
+  rc = make_tmap(&tb, B, obb, 64, B_MN ? 64 : BN);
   if (rc) return rc;
   if ((rc = make_second_pair(&ta2, &tb2, A2, B2, s.batches, TC_BM, BN, A_MN, B_MN))) return rc;
   GemmEpilogue e = e_in;
@@ -1719,10 +1720,11 @@ int launch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Oper
                const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = Tc2Config;
   CUtensorMap ta, tb, ta2, tb2, tout, taux;
-  const int ob = s.parts ? 3 : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int ob = s.parts ? (s.parts == 6 ? 3 : 2) : s.ksplit > 1 ? 1 : s.batches;  // split-K operands are not batched
+  const int obb = s.parts == 2 ? 1 : ob;
   int rc = make_tmap(&ta, A, ob, 64, A_MN ? 64 : 128);
   if (rc) return rc;
-  rc = make_tmap(&tb, B, ob, 64, B_MN ? 64 : 128);
+  rc = make_tmap(&tb, B, obb, 64, B_MN ? 64 : 128);
   if (rc) return rc;
   if ((rc = make_second_pair(&ta2, &tb2, A2, B2, s.batches, 128, 128, A_MN, B_MN))) return rc;
   GemmEpilogue e = e_in;
@@ -1830,7 +1832,7 @@ int run_gemm2(const Operand& A, const Operand& B, const Operand* A2, const Opera
   ULM_REQUIRE(s.ksplit <= 1 || (s.causal == CAUSAL_NONE && s.ksplit == s.batches &&
                                  (int64_t)(s.ksplit - 1) * ksplit_chunk(s.K, s.ksplit) < s.K),
               "split K needs a non-causal product, batches == ksplit and no empty k range");
-  ULM_REQUIRE(!s.parts || (A.dtype == ULM_BF16 && (s.batches == 1 || s.ksplit > 1) && s.K2 == 0 && !s.carry &&
+  ULM_REQUIRE(!s.parts || ((s.parts == 6 || s.parts == 2) && A.dtype == ULM_BF16 && (s.batches == 1 || s.ksplit > 1) && s.K2 == 0 && !s.carry &&
                            s.causal == CAUSAL_NONE),
               "operand parts need a plain product of bf16 parts");
   if (s.batches == 0 || s.M == 0 || s.N == 0) return ULM_OK;

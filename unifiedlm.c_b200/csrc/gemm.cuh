@@ -57,13 +57,16 @@ struct GemmShape {
   // fp32 FMA back end: 1 = one running sum over k in order (run.c's matmul order, for the decode
   // steps' token identity); 0 = each 16-deep k slice summed apart, then added (smaller rounding)
   int k_in_order = 0;
-  // > 0: fp32 operands as three bf16 parts each (hi, mid, lo: batches 0, 1, 2 of A and B, one output
-  // batch, or one for each range of ksplit); the k range is walked once for each of the six pairs GEMM_PART_A / GEMM_PART_B, the small
-  // products first. Left out are the products below 2^-25 of the whole one.
+  // > 0: operands in bf16 parts (hi first), which are their batches (one output batch, or one for each
+  // range of ksplit); the k range is walked once for each pair of parts, the small products first.
+  // 6: fp32 operands, three parts each (hi, mid, lo), pairs GEMM_PART_A / GEMM_PART_B; left out are the
+  // products below 2^-25 of the whole one. 2: A has two parts, B is whole.
   int parts = 0;
 };
 __device__ constexpr int GEMM_PART_A[6] = {2, 0, 1, 1, 0, 0};
 __device__ constexpr int GEMM_PART_B[6] = {0, 2, 1, 0, 1, 0};
+__device__ __forceinline__ int gemm_part_a(int parts, int i) { return parts == 6 ? GEMM_PART_A[i] : parts - 1 - i; }
+__device__ __forceinline__ int gemm_part_b(int parts, int i) { return parts == 6 ? GEMM_PART_B[i] : 0; }
 
 // Chunk steps a carry tile runs.
 __host__ __device__ inline int carry_steps(const GemmShape& s) {

@@ -586,7 +586,14 @@ int lp_check_top(int64_t N, int64_t V, int k, const int64_t* top_ids, const floa
 
 bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
-constexpr int LP_MAX_K_SPLITS = 4;
+constexpr int LP_MAX_K_SPLITS = 32;
+
+// bf16 parts of the logits' gradient in bf16 precision. One part rounds each of its values by up to 2^-9
+// on the way to dh and dW, which with bf16 results makes their error 1.4 times that of the results' own
+// rounding (0.0024 against 0.0017), and up to twice that where few rows leave little to average (7 rows:
+// 0.0033). Two parts cost another pass of both products (V = 32000, D = 768: 81 -> 95 us for 256 rows, 100 ->
+// 140 for 512).
+int lp_parts(int64_t N) { return N <= 256 ? 2 : 1; }
 constexpr int64_t LP_DUMP_BYTES = 256ll << 20;
 
 // How the head's forward finds the alternatives: from register lists of chunks where the rows are so many
@@ -624,7 +631,7 @@ int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
     const double round_us = 2.0 * 256 * 256 * (double)k / 19e6;   // of all pairs, at 1400 TFLOP/s
     const double part_us = (double)rows * (double)D * 8 / 6.5e6;  // a partial sum, written and read
     double least = (double)cdiv(tiles, pairs) * round_us;
-    for (int c = 2; c <= LP_MAX_K_SPLITS && c * 4096 <= k; ++c) {
+    for (int c = 2; c <= LP_MAX_K_SPLITS && c * 512 <= k; ++c) {
       const double t = (double)cdiv(tiles * c, pairs) / c * round_us + c * part_us + 5.0;
       if (t < least) {
         least = t;
@@ -657,7 +664,7 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     w.w_parts = take(3 * V * ldd * 2);
   }
   if (backward) {
-    w.dx = take(N * ldv * (f32 ? 4 : 2));
+    w.dx = take(N * ldv * (f32 ? 4 : 2 * lp_parts(N)));
     if (f32)
       w.dx_parts = take(3 * N * ldv * 2);
     else  // partial sums of dh, then of dW
@@ -809,7 +816,8 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   CUtensorMap th, tw, to;
   if (int rc = lp_operand(&th, h_op, ld_h, N, D, f32, w.h_parts, st)) return rc;
   if (int rc = lp_operand(&tw, w_op, ld_w, V, D, f32, w.w_parts, st)) return rc;
-  ULM_REQUIRE(make_epi_tmap(&to, EPI_MODE_WARP, w.dx, f32 ? ULM_F32 : ULM_BF16, V, N, 1, ldv, N * ldv),
+  const int parts = f32 ? 1 : lp_parts(N);
+  ULM_REQUIRE(make_epi_tmap(&to, EPI_MODE_WARP, w.dx, f32 ? ULM_F32 : ULM_BF16, V, N, parts, ldv, N * ldv),
               "no tensor map of the logits' gradient");
   LpArgs a{};
   a.tokens = tokens;
@@ -817,6 +825,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   a.entropy = entropy;
   a.dlogprobs = dlogprobs;
   a.dentropy = dentropy;
+  a.parts = parts;
   if (int rc = f32 ? lp_launch<LP_GRAD, 0, true>(th, tw, to, s, a, st) : lp_launch<LP_GRAD, 0, false>(th, tw, to, s, a, st))
     return rc;
   const void *dx = w.dx, *hh = h_op, *ww = w_op;
@@ -832,7 +841,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   // replaced.
   auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) -> int {
     GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
-    g.parts = f32 ? 6 : 0;
+    g.parts = f32 ? 6 : parts == 2 ? 2 : 0;
     const int splits = lp_splits(rows, k, D, f32, f32 ? N * ldv : 0);
     if (splits <= 1) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
     g.batches = g.ksplit = splits;

@@ -96,6 +96,7 @@ struct LpArgs {
   const float* entropy;
   const float* dlogprobs;
   const float* dentropy;
+  int parts;  // bf16 parts of the gradient: 1, or 2 (hi and lo, the output map's batches)
 };
 
 // The backward's factors of one row: dx_v = [v = t] a - p_v (a + b (log p_v + H)), with p_v = 2^l,
@@ -462,7 +463,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         for (int i = 0; i < nch; ++i) {
           uint8_t* out = slots + (n % LPM_SLOTS) * 4096;
           ++n;
-          if (lane == 0) bulk_wait_group_read<LPM_SLOTS - 1>();  // the store before last has read its slot
+          const bool two = !F32 && args.parts == 2;
+          if (lane == 0) {
+            if (two)
+              bulk_wait_group_read<0>();  // both slots are taken
+            else
+              bulk_wait_group_read<LPM_SLOTS - 1>();  // the store before last has read its slot
+          }
           __syncwarp();
 #pragma unroll
           for (int hh = 0; hh < CW / 32; ++hh) {
@@ -478,11 +485,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             }
             __syncwarp();
             stage_write<F32, 32>(out, lane, hh * (F32 ? 8 : 4), v);
+            if (two) {
+#pragma unroll
+              for (int q = 0; q < 32; ++q) v[q] -= __bfloat162float(__float2bfloat16_rn(v[q]));
+              stage_write<F32, 32>(slots + (n % LPM_SLOTS) * 4096, lane, hh * 4, v);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_3d(&tma_out, out, col_base + i * CW, tile.rb * 256 + (int)rank * 128 + quad * 32, 0);
+            const int r0 = tile.rb * 256 + (int)rank * 128 + quad * 32;
+            tma_store_3d(&tma_out, out, col_base + i * CW, r0, 0);
+            if (two) tma_store_3d(&tma_out, slots + (n % LPM_SLOTS) * 4096, col_base + i * CW, r0, 1);
             bulk_commit_group();
           }
         }
