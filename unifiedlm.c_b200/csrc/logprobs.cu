@@ -39,12 +39,15 @@ __device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b) {
   return a;
 }
 
-// NV more logits into a thread's statistics: the largest and the smallest first. Where a logit is below
-// -1e30 (-inf, or the type's lowest value, is a mask) its term is left out: 2^(.) is 0, but (.) may be
-// -inf.
+// NV more logits into a thread's statistics: the largest and the smallest first. Logits below -1e30 (-inf,
+// or the type's lowest value, is a mask) count as -1e35, whose power is 0 too, but whose product with it is
+// no 0 times -inf.
 // Returns the largest, or +inf once the sum is NaN.
 template <int NV>
-__device__ __forceinline__ float lp_add(LpStat& st, const float (&x)[NV]) {
+__device__ __forceinline__ float lp_add(LpStat& st, const float (&given)[NV]) {
+  float x[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) x[i] = given[i];
   float hi = x[0], lo = x[0];
 #pragma unroll
   for (int i = 1; i < NV; ++i) {
@@ -54,12 +57,7 @@ __device__ __forceinline__ float lp_add(LpStat& st, const float (&x)[NV]) {
   if (hi > st.m) st.raise(hi);
   if (lo < LP_LEAST) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float d = fmaf(x[i], LOG2E, -st.m2), e = fast_exp2(d);
-      st.s += e;
-      st.u = e > 0.f ? fmaf(e, d, st.u) : st.u;
-    }
-    return st.s == st.s ? hi : INFINITY;
+    for (int i = 0; i < NV; ++i) x[i] = x[i] < LP_LEAST ? -1e35f : x[i];
   }
   float s1 = 0.f, u1 = 0.f;
   if (NV % 2 == 0) {
