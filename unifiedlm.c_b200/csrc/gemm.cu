@@ -750,7 +750,9 @@ struct TcConfig {
   static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + epi_smem_bytes(EPI_SLOTS) + 1024 + 512;
 };
 
-template <int BN, bool A_MN, bool B_MN>
+// PARTS: operands in bf16 parts (GemmShape.parts), an instance of its own so that the others' producer loop
+// stays as short as it was
+template <int BN, bool A_MN, bool B_MN, bool PARTS>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     tc_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                    const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
@@ -867,7 +869,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
         const int n1 = kb1 - kb0;
-        const int nkb = shape.parts ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = PARTS ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         for (int i = 0; i < nkb; ++i) {
           if (!wait_or_abort(&empty[stage], phase ^ 1u, abort_flag, DEVERR_GEMM_PRODUCER_WAIT)) {
@@ -878,13 +880,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           uint8_t* sb = sa + Cfg::A_BYTES;
           mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
           // k blocks of the first operand pair, then those of the second (shape.K2)
-          const int part = shape.parts ? i / n1 : 0;  // pair of operand parts (shape.parts)
-          const bool s2 = !shape.parts && i >= n1;
+          const int part = PARTS ? i / n1 : 0;  // pair of operand parts
+          const bool s2 = !PARTS && i >= n1;
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
           const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
-          const int oa = shape.parts ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = shape.parts ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int oa = PARTS ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = PARTS ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d(ma, sa, &full[stage], k0, tc.mb * TC_BM, oa);
           } else {
@@ -963,7 +965,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<TC_BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = shape.parts ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = PARTS ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1048,7 +1050,7 @@ struct Tc2Config {
   static constexpr uint32_t SMEM_BYTES = TC2_STAGES * STAGE_BYTES + epi_smem_bytes(EPI_SLOTS) + 1024 + 512;
 };
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
     tc2_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                     const __grid_constant__ CUtensorMap tma_a2, const __grid_constant__ CUtensorMap tma_b2,
@@ -1172,7 +1174,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
         const int n1 = kb1 - kb0;
-        const int nkb = shape.parts ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = PARTS ? shape.parts * n1 : n1 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int ob = shape.ksplit > 1 ? 0 : tc.b;  // operand batch coordinate
         const int row0 = tc.mb * BM + (int)rank * 128;
         const int col0 = tc.nb * BN + (int)rank * 128;
@@ -1186,13 +1188,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
           const uint32_t bar = leader_full + (uint32_t)(stage * sizeof(uint64_t));
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
           // k blocks of the first operand pair, then those of the second (shape.K2)
-          const int part = shape.parts ? i / n1 : 0;  // pair of operand parts (shape.parts)
-          const bool s2 = !shape.parts && i >= n1;
+          const int part = PARTS ? i / n1 : 0;  // pair of operand parts
+          const bool s2 = !PARTS && i >= n1;
           const CUtensorMap* ma = s2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mbm = s2 ? &tma_b2 : &tma_b;
           const int k0 = (s2 ? i - n1 : kb0 + i - part * n1) * TC_BK;
-          const int oa = shape.parts ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
-          const int obb = shape.parts ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
+          const int oa = PARTS ? gemm_part_a(shape.parts, part) : s2 ? (shape.a2_batched ? tc.b : 0) : ob;
+          const int obb = PARTS ? gemm_part_b(shape.parts, part) : s2 ? (shape.b2_batched ? tc.b : 0) : ob;
           if (!A_MN) {
             tma_load_3d_pair(ma, sa, bar, k0, row0, oa);
           } else {
@@ -1268,7 +1270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         if (t < 0) continue;
         const TileCoord tc = decode_tile<BM, BN>(t, shape, m_blocks, n_blocks, tiles_per_batch);
         const int kb0 = tc.k_begin / TC_BK, kb1 = (tc.k_end + TC_BK - 1) / TC_BK;
-        const int nkb = shape.parts ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
+        const int nkb = PARTS ? shape.parts * (kb1 - kb0) : kb1 - kb0 + (shape.K2 + TC_BK - 1) / TC_BK;
         const int jj = j++;
         const int acc = jj & 1;
         const uint32_t acc_phase = (uint32_t)(jj >> 1) & 1u;
@@ -1669,7 +1671,7 @@ int make_second_pair(CUtensorMap* ta2, CUtensorMap* tb2, const Operand* A2, cons
   return make_tmap(tb2, *B2, B2->bstride ? batches : 1, 64, b_mn ? 64 : b_rows);
 }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool A_MN, bool B_MN, bool PARTS = false>
 int launch_tc(const Operand& A, const Operand& B, const Operand* A2, const Operand* B2, const GemmShape& s,
               const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = TcConfig<BN>;
@@ -1690,7 +1692,7 @@ int launch_tc(const Operand& A, const Operand& B, const Operand* A2, const Opera
     return ULM_ERR_INVALID;
   }
   if (!configured[dev]) {
-    ULM_CUDA_TRY(cudaFuncSetAttribute(tc_gemm_kernel<BN, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    ULM_CUDA_TRY(cudaFuncSetAttribute(tc_gemm_kernel<BN, A_MN, B_MN, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)Cfg::SMEM_BYTES));
     configured[dev] = true;
   }
@@ -1702,20 +1704,23 @@ int launch_tc(const Operand& A, const Operand& B, const Operand* A2, const Opera
   if (total == 0) return ULM_OK;
   const int grid = total < sm_count(dev) ? total : sm_count(dev);
   const GemmShape sb = with_schedule(s, total, grid);
-  return launch_pdl(tc_gemm_kernel<BN, A_MN, B_MN>, dim3(grid), dim3(TC_THREADS), Cfg::SMEM_BYTES, st, ta, tb, ta2,
+  return launch_pdl(tc_gemm_kernel<BN, A_MN, B_MN, PARTS>, dim3(grid), dim3(TC_THREADS), Cfg::SMEM_BYTES, st, ta, tb, ta2,
                     tb2, tout, taux, sb, e, m_blocks, n_blocks, tpb, total);
 }
 
 template <int BN>
 int dispatch_tc_major(const Operand& A, const Operand& B, const Operand* A2, const Operand* B2, const GemmShape& s,
                       const GemmEpilogue& e, cudaStream_t st) {
+  if (s.parts)
+    return A.mn_major ? launch_tc<BN, true, true, true>(A, B, A2, B2, s, e, st)
+                      : launch_tc<BN, false, true, true>(A, B, A2, B2, s, e, st);
   if (!A.mn_major && !B.mn_major) return launch_tc<BN, false, false>(A, B, A2, B2, s, e, st);
   if (!A.mn_major && B.mn_major) return launch_tc<BN, false, true>(A, B, A2, B2, s, e, st);
   if (A.mn_major && !B.mn_major) return launch_tc<BN, true, false>(A, B, A2, B2, s, e, st);
   return launch_tc<BN, true, true>(A, B, A2, B2, s, e, st);
 }
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool PARTS = false>
 int launch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Operand* B2, const GemmShape& s,
                const GemmEpilogue& e_in, cudaStream_t st) {
   using Cfg = Tc2Config;
@@ -1736,7 +1741,7 @@ int launch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Oper
     return ULM_ERR_INVALID;
   }
   if (!configured[dev]) {
-    ULM_CUDA_TRY(cudaFuncSetAttribute(tc2_gemm_kernel<A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    ULM_CUDA_TRY(cudaFuncSetAttribute(tc2_gemm_kernel<A_MN, B_MN, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)Cfg::SMEM_BYTES));
     configured[dev] = true;
   }
@@ -1749,12 +1754,15 @@ int launch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Oper
   const int max_pairs = sm_count(dev) / 2;
   const int pairs = total < max_pairs ? total : max_pairs;
   const GemmShape sb = with_schedule(s, total, pairs);
-  return launch_pdl(tc2_gemm_kernel<A_MN, B_MN>, dim3(2 * pairs), dim3(TC_THREADS), Cfg::SMEM_BYTES, st, ta, tb, ta2,
+  return launch_pdl(tc2_gemm_kernel<A_MN, B_MN, PARTS>, dim3(2 * pairs), dim3(TC_THREADS), Cfg::SMEM_BYTES, st, ta, tb, ta2,
                     tb2, tout, taux, sb, e, m_blocks, n_blocks, tpb, total);
 }
 
 int dispatch_tc2(const Operand& A, const Operand& B, const Operand* A2, const Operand* B2, const GemmShape& s,
                  const GemmEpilogue& e, cudaStream_t st) {
+  if (s.parts)
+    return A.mn_major ? launch_tc2<true, true, true>(A, B, A2, B2, s, e, st)
+                      : launch_tc2<false, true, true>(A, B, A2, B2, s, e, st);
   if (!A.mn_major && !B.mn_major) return launch_tc2<false, false>(A, B, A2, B2, s, e, st);
   if (!A.mn_major && B.mn_major) return launch_tc2<false, true>(A, B, A2, B2, s, e, st);
   if (A.mn_major && !B.mn_major) return launch_tc2<true, false>(A, B, A2, B2, s, e, st);
@@ -1833,8 +1841,8 @@ int run_gemm2(const Operand& A, const Operand& B, const Operand* A2, const Opera
                                  (int64_t)(s.ksplit - 1) * ksplit_chunk(s.K, s.ksplit) < s.K),
               "split K needs a non-causal product, batches == ksplit and no empty k range");
   ULM_REQUIRE(!s.parts || ((s.parts == 6 || s.parts == 2) && A.dtype == ULM_BF16 && (s.batches == 1 || s.ksplit > 1) && s.K2 == 0 && !s.carry &&
-                           s.causal == CAUSAL_NONE),
-              "operand parts need a plain product of bf16 parts");
+                           s.causal == CAUSAL_NONE && B.mn_major),
+              "operand parts need a plain product of bf16 parts, B in [k][n] order");
   if (s.batches == 0 || s.M == 0 || s.N == 0) return ULM_OK;
   ULM_REQUIRE(s.K > 0, "empty contraction");
   if (A.dtype == ULM_BF16) {

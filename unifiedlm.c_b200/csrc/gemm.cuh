@@ -61,6 +61,7 @@ struct GemmShape {
   // range of ksplit); the k range is walked once for each pair of parts, the small products first.
   // 6: fp32 operands, three parts each (hi, mid, lo), pairs GEMM_PART_A / GEMM_PART_B; left out are the
   // products below 2^-25 of the whole one. 2: A has two parts, B is whole.
+  // B is MN-major.
   int parts = 0;
 };
 __device__ constexpr int GEMM_PART_A[6] = {2, 0, 1, 1, 0, 0};
