@@ -167,3 +167,9 @@ def test_refusals():
     for a in ((t.float(), w), (t, w.half()), (t.bool(), w)):
         with pytest.raises(TypeError):
             embedding(*a)
+
+
+def test_second_derivatives_are_refused():
+    w = torch.randn(5, 4, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(embedding(torch.zeros(3, dtype=torch.long, device="cuda"), w).sum(), w, create_graph=True)

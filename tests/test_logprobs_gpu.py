@@ -457,3 +457,64 @@ def test_head_rows_of_nan():
         assert r.top_ids[1].tolist() == list(range(k))
         keep = torch.arange(N, device="cuda") != 1
         assert all(torch.equal(a[keep], b[keep]) for a, b in zip(r, want))
+
+
+def test_two_calls_at_once():
+    """The same kernels on two streams at the same time, each with its own inputs and workspaces."""
+    cases = [head_inputs(N, V, D, torch.bfloat16, N)[:3] for N, V, D in ((900, 4000, 128), (40, 30000, 96))]
+    xs = [torch.randn(N, V, device="cuda") for N, V in ((300, 9000), (2, 32000))]
+
+    def one(h, w, t, x):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        r = lm_head_logprobs(h, w, t, top_k=7)
+        g = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), [h, w])
+        s = token_logprobs(x, torch.arange(x.shape[0], device="cuda"), top_k=7)
+        return [*r, *g, *s]
+
+    want = [[o.detach().clone() for o in one(*c, x)] for c, x in zip(cases, xs)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, c, x in zip(streams, cases, xs):
+            with torch.cuda.stream(s):
+                got.append(one(*c, x))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+    assert L.device_error() == 0
+
+
+def test_captured_training_step():
+    """Forward and backward in one graph, captured while no eager graph of the same leaves lives, replayed
+    with new inputs in place."""
+    for N, V, D, dt in ((70, 900, 64, torch.bfloat16), (300, 700, 40, torch.float32)):
+        h, w, t, _ = head_inputs(N, V, D, dt, N)
+        h, w = h.requires_grad_(), w.requires_grad_()
+        x = torch.randn(N, V, device="cuda").to(dt).requires_grad_()
+        prec = "bf16" if dt == torch.bfloat16 else "fp32"
+
+        def step():
+            r, s = lm_head_logprobs(h, w, t, precision=prec), token_logprobs(x, t)
+            return torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + s.logprobs.sum() + s.entropy.sum(), [h, w, x])
+
+        step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        for _ in range(2):
+            with torch.no_grad():
+                h.normal_(), x.normal_()
+            g.replay()
+            got = [o.clone() for o in out]
+            assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 40, device="cuda", requires_grad=True)
+    w = torch.randn(50, 40, device="cuda", requires_grad=True)
+    t = torch.zeros(3, dtype=torch.long, device="cuda")
+    for out in (token_logprobs(x, t).logprobs, lm_head_logprobs(x, w, t).entropy):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)

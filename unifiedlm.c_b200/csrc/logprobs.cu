@@ -238,7 +238,7 @@ __device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* red) {
 // its logits for the statistics and, for the alternatives, a second look at those batches whose maximum
 // reaches a threshold: the k-th largest of 64 groups' maxima bounds the k-th best logit of the run from
 // below, and only about k logits reach it. The cluster's first CTA joins the runs. Bound by the pass over HBM for
-// many rows (4096 x 32000 bf16: 63 us, 4.1 TB/s), by latency for few: a row of 32000 split over 8 CTAs takes
+// many rows (4096 x 32000 bf16: 58 us, 4.5 TB/s), by latency for few: a row of 32000 split over 8 CTAs takes
 // 10 us, on one CTA 15.5 us.
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
@@ -444,7 +444,7 @@ __device__ __forceinline__ void lp_store<__nv_bfloat16>(__nv_bfloat16* p, float 
 }
 
 // Elementwise: CTA (row, run of LP_BWD_RUN columns). 16-byte pieces where both rows have the same place
-// in theirs, else one logit at a time. Bound by HBM (read and write).
+// in theirs, else one logit at a time. Bound by HBM (read and write; 4096 x 32000 bf16: 86 us, 6.1 TB/s).
 constexpr int LP_BWD_RUN = 16384;
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS)
@@ -595,13 +595,12 @@ int lp_parts(int64_t N) { return N <= 256 ? 2 : 1; }
 constexpr int64_t LP_DUMP_BYTES = 256ll << 20;
 
 // How the head's forward finds the alternatives: from register lists of chunks where the rows are so many
-// that the epilogue sees a row long enough to keep its list for most chunks, or from the logits themselves,
-// written out for as many rows at a time as 256 MB hold. At V = 32000, D = 768, k = 8 lists take 119 us for
-// 2048 rows and 192 for 4096, written out 120 and 243; k = 20 lists 294 us for 4096 rows and 797 for 16384,
-// written out 251 and 1014.
-bool lp_lists(int64_t N, int64_t V, int k) {
-  return k > 0 && N * V > (k <= LP_LIST ? 2048ll * 32000 : 8192ll * 32000);
-}
+// for k that the epilogue sees a row long enough to keep its list for most chunks, or from the logits
+// themselves, written out for as many rows at a time as 256 MB hold. Lists against written out at V = 32000,
+// D = 768, us: k = 1, 1024 rows 51 and 63 (333 rows x 288: 30 and 29); k = 8, 1024 rows 80 and 65, 2048 116
+// and 119, 4096 185 and 245; k = 20, 4096 rows 294 and 265, 8192 520 and 555; k = 32, 8192 rows 630 and 570,
+// 16384 1075 and 1177.
+bool lp_lists(int64_t N, int64_t V, int k) { return k > 0 && N * V > 320ll * k * 32000; }
 int64_t lp_ld_max(int64_t V) { return cdiv(V, 256) * 8; }  // chunks of whole tiles
 int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
   if (k == 0 || lp_lists(N, V, k)) return N;

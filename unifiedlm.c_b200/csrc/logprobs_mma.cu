@@ -8,8 +8,8 @@
 // comparison for 32 logits. For many rows an epilogue thread keeps a sorted list of the k best chunks of its
 // share and writes a chunk that enters the list to the place of the one that leaves it (about
 // k ln(chunks / k) times). LP_DUMP, for few rows, where most chunks of the short shares would enter, writes
-// all logits and the maxima of the chunks, and lp_join_kernel picks (2048 x 32000 x 768, k = 20: lists 188
-// us, written out 125; 16384 rows: 797 and 1014; no alternatives: 75 and 561).
+// all logits and the maxima of the chunks, and lp_join_kernel picks (2048 x 32000 x 768, k = 20: lists 191
+// us, written out 124; 16384 rows: 920 and 1140; no alternatives: 70 and 535, 1500 TFLOP/s).
 // LP_GRAD writes the logits' gradient ([v = t] a - p (a + b (log p + H))) in the operand type of the
 // products that follow.
 //
