@@ -648,33 +648,33 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
   };
   int best = 0;
   if (!DUMP) {
-  sync();
-  const int heads = counts[w][0], lists = min(heads, k);
-  rank(heads, [&](int c, int r) {
-    chosen[w][r] = at[c];
-    if (r == k - 1) bound[w] = key[c];
-  });
-  sync();
-  const uint64_t floor_key = heads >= k ? bound[w] : 0;  // the k-th best first chunk
-  // the chosen lists' chunks that are not under it
+    sync();
+    const int heads = counts[w][0], lists = min(heads, k);
+    rank(heads, [&](int c, int r) {
+      chosen[w][r] = at[c];
+      if (r == k - 1) bound[w] = key[c];
+    });
+    sync();
+    const uint64_t floor_key = heads >= k ? bound[w] : 0;  // the k-th best first chunk
+    // the chosen lists' chunks that are not under it
 #pragma unroll 4
-  for (int i = tid; i < lists * 32; i += TPR) {
-    const int l = chosen[w][i / 32], j = i % 32;
-    if (j >= k) continue;
-    const float2 e = list[(int64_t)l * k + j];
-    const int id = __float_as_int(e.y);
-    const uint64_t kk = lp_key(e.x, (uint32_t)(id >> 5));
-    if (id >= 0 && kk >= floor_key) {
-      const int to = atomicAdd(&counts[w][1], 1);
-      key[to] = kk;
-      at[to] = l * k + (id & 31);
+    for (int i = tid; i < lists * 32; i += TPR) {
+      const int l = chosen[w][i / 32], j = i % 32;
+      if (j >= k) continue;
+      const float2 e = list[(int64_t)l * k + j];
+      const int id = __float_as_int(e.y);
+      const uint64_t kk = lp_key(e.x, (uint32_t)(id >> 5));
+      if (id >= 0 && kk >= floor_key) {
+        const int to = atomicAdd(&counts[w][1], 1);
+        key[to] = kk;
+        at[to] = l * k + (id & 31);
+      }
     }
-  }
-  sync();
-  const int chunks = counts[w][1];
-  best = min(chunks, k);
-  rank(chunks, [&](int c, int r) { chosen[w][r] = c; });
-  sync();
+    sync();
+    const int chunks = counts[w][1];
+    best = min(chunks, k);
+    rank(chunks, [&](int c, int r) { chosen[w][r] = c; });
+    sync();
   } else {
     const int chunks = (shape.V + 31) / 32;
     const float* cm = args.chunk_max + row * args.ld_max;

@@ -69,8 +69,8 @@ def lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision, stats=True):
     lib = L.lib()
     out = lp, ent, st, ids, tlp = _outputs(N, top_k, h.device, stats)
     opt = _op_dtype(precision)
-    h_op, ld_h = _operand(h.detach(), opt)
-    w_op, ld_w = _operand(weight.detach(), opt)
+    h_op, ld_h = _operand(h, opt)
+    w_op, ld_w = _operand(weight, opt)
     work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, top_k, 0, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
         L.check(lib.ulm_lm_head_logprobs_fwd(h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(),
@@ -87,8 +87,8 @@ def lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision
     dh = torch.empty(N, D, device=h.device, dtype=h.dtype) if need_dh else None
     dw = torch.empty(V, D, device=h.device, dtype=weight.dtype) if need_dw else None
     opt = _op_dtype(precision)
-    h_op, ld_h = _operand(h.detach(), opt)
-    w_op, ld_w = _operand(weight.detach(), opt)
+    h_op, ld_h = _operand(h, opt)
+    w_op, ld_w = _operand(weight, opt)
     work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, 1, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
         L.check(lib.ulm_lm_head_logprobs_bwd(
