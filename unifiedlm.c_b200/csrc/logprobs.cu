@@ -612,8 +612,9 @@ int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
 // Ranges of k into which the product (rows x D) over k of the backward is split.
 //
 // The tensor cores cut off what an accumulator cannot hold, a little with each step of 16 in k, always
-// towards zero: fp32 products are taken over ranges of about 512, as far as `room` floats hold their sums,
-// which are added with rounding (at 1001 x 4099 x 288 the gradients' error falls from 8e-6 to 1e-6).
+// towards zero: fp32 products are taken over ranges of about 256, as far as `room` floats hold their sums,
+// which are added with rounding (at 1001 x 4099 x 288 the gradients' error falls from 8e-6 to 5e-7; ranges
+// of 512 have 1e-6 and take 95 instead of 101 us there, 73 instead of 65 at 16 x 1416 x 768).
 //
 // A bf16 product whose 256 x 256 tiles fill the CTA pairs badly (8192 x 768: 96 tiles, two rounds of 74) is
 // split where the rounds saved are worth writing and adding the partial sums (that one over 32000: 346 us,
@@ -621,7 +622,7 @@ int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
 int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
   int splits = 1;
   if (f32) {
-    splits = (int)std::min<int64_t>(room / (rows * D), cdiv(k, 512));
+    splits = (int)std::min<int64_t>(room / std::max<int64_t>(1, rows * D), cdiv(k, 256));
   } else {
     const int pairs = lp_sms() / 2;
     const int64_t tiles = cdiv(rows, 256) * cdiv(D, 256);
@@ -638,6 +639,13 @@ int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
   }
   return splits > 1 ? (int)cdiv(k, ksplit_chunk((int)k, splits)) : 1;  // no empty range
 }
+
+// Floats for an fp32 product's sums: 64 MB of them, or the place of the fp32 gradient of the logits, which
+// its parts have replaced by then, where that is larger (that place alone would hold too few of them where the
+// vocabulary is little wider than the model: 16 x 1416 x 768 107 us and an error of 2.7e-6, now 65 and 5e-7;
+// 1000 x 1500 x 1024 146 and 2.9e-6, now 117 and 5e-7).
+constexpr int64_t LP_SUMS = 16ll << 20;
+int64_t lp_room(int64_t N, int64_t V) { return std::max(N * ulm_operand_ld(V), LP_SUMS); }
 
 // The work buffer of the head's entries.
 struct LpWork {
@@ -662,10 +670,13 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
   }
   if (backward) {
     w.dx = take(N * ldv * (f32 ? 4 : 2 * lp_parts(N)));
-    if (f32)
-      w.dx_parts = take(3 * N * ldv * 2);
-    else  // partial sums of dh, then of dW
-      w.sums = floats(std::max(lp_splits(N, V, D, false, 0) * N, lp_splits(V, N, D, false, 0) * V) * D);
+    if (f32) w.dx_parts = take(3 * N * ldv * 2);
+    // partial sums of dh, then of dW
+    const int64_t room = lp_room(N, V);
+    if (f32 && room > LP_SUMS)
+      w.sums = static_cast<float*>(w.dx);
+    else
+      w.sums = floats(std::max(lp_splits(N, V, D, f32, room) * N, lp_splits(V, N, D, f32, room) * V) * D);
   } else {
     const int64_t rows = lp_rows_at_once(N, V, k);
     // the shares of the rows of one launch: all of them, but for the last one's fewer rows
@@ -833,19 +844,16 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
     ww = w.w_parts;
     ld_h = ld_w = ldd;
   }
-  // Each product's operands are single matrices, or the three parts of one (its batches); its partial sums
-  // (lp_splits) of fp32 operands take the place of the fp32 gradient of the logits, which its parts have
-  // replaced.
+  // each product's operands are single matrices, or the parts of one (its batches)
   auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) -> int {
     GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
     g.parts = f32 ? 6 : parts == 2 ? 2 : 0;
-    const int splits = lp_splits(rows, k, D, f32, f32 ? N * ldv : 0);
+    const int splits = lp_splits(rows, k, D, f32, lp_room(N, V));
     if (splits <= 1) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
     g.batches = g.ksplit = splits;
-    float* sums = f32 ? static_cast<float*>(w.dx) : w.sums;
-    if (int rc = run_gemm(A, B, g, make_epilogue(EPI_STORE, ULM_F32, sums, D, rows * D, nullptr), st)) return rc;
+    if (int rc = run_gemm(A, B, g, make_epilogue(EPI_STORE, ULM_F32, w.sums, D, rows * D, nullptr), st)) return rc;
     return launch_pdl(lp_add_kernel, dim3((unsigned)std::min<int64_t>(cdiv(rows * D, 1024), 1 << 20)), dim3(256), 0, st,
-                      static_cast<const float*>(sums), splits, rows * D, out, dtype);
+                      static_cast<const float*>(w.sums), splits, rows * D, out, dtype);
   };
   if (dh) {
     // dh = dx W: A = dx (rows, K-major over the vocabulary), B = W as [token][d] (MN-major)
