@@ -1,0 +1,51 @@
+"""The log-probability entries at their edges: digits of the gradients, alternatives of rows in order,
+many small calls one after another, rows with NaN, tokens out of range. Oracles in float64."""
+import pytest
+import torch
+
+import unifiedlm_c_b200._lib as L
+from unifiedlm_c_b200.logprobs import lm_head_logprobs
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def on_grid(N, V, D, seed, dtype):
+    """Operands in whole steps that bf16 holds, so that each logit is exact in fp32, whatever the order
+    of its sum: products are multiples of 2^-9 below 2^2, a thousand of them below 2^12."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    h = (torch.randn(N, D, device="cuda", generator=gen) * 4).round().clamp(-15, 15) / 8
+    w = (torch.randn(V, D, device="cuda", generator=gen) * 3).round().clamp(-15, 15) / 64
+    t = torch.randint(-1, V, (N,), device="cuda", generator=gen)
+    return h.to(dtype), w.to(dtype), t, gen
+
+
+@pytest.mark.parametrize("N,V,D", [(1, 300, 64), (256, 1000, 64), (257, 1000, 64), (700, 2050, 96), (2049, 515, 40)])
+def test_head_backward_holds_the_logits_gradient_in_16_digits(N, V, D):
+    """bf16 operands held in fp32 tensors: dh and dw come in fp32, and with the logits exact their only
+    errors are those of the statistics, of the logits' gradient in two bf16 parts (each value off by 2^-17)
+    and of the fp32 sums. One bf16 part (2^-8 a value) is a hundred times past the bound."""
+    h, w, t, gen = on_grid(N, V, D, N, torch.float32)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    a = torch.randn(N, device="cuda", generator=gen)
+    b = torch.randn(N, device="cuda", generator=gen)
+    r = lm_head_logprobs(h, w, t, precision="bf16")
+    dh, dw = torch.autograd.grad([r.logprobs, r.entropy], [h, w], [a, b])
+    assert dh.dtype == torch.float32 and dw.dtype == torch.float32
+    h64, w64, a, b = h.detach().double(), w.detach().double(), a.double(), b.double()
+    logp = torch.log_softmax(h64 @ w64.t(), -1)
+    p = logp.exp()
+    ent = -(p * logp).sum(-1)
+    a = torch.where(t >= 0, a, 0.0)
+    d = -p * (a[:, None] + b[:, None] * (logp + ent[:, None]))
+    size = p * (a.abs()[:, None] + b.abs()[:, None] * (logp.abs() + ent[:, None]))
+    d = d.scatter_add(1, t.clamp(min=0)[:, None], a[:, None])
+    # the statistics: sums of V powers, each of them off by 2^-22 and by its argument's rounding (up to 40 log2 e)
+    rs = (V / 32 + 32) * U + 2.0 ** -22 + 80 * U
+    d_err = size * 8 * rs + (d.abs() + size) * 2.0 ** -17
+    for got, want, err, mag, n in ((dh, d @ w64, d_err @ w64.abs(), d.abs() @ w64.abs(), V),
+                                   (dw, d.t() @ h64, d_err.t() @ h64.abs(), d.abs().t() @ h64.abs(), N)):
+        # sums of n products of two parts, in steps of 16 that may each cut off 2u
+        tol = err + (n / 16 + 16) * 4 * U * mag + 1e-30
+        assert bool(((got.double() - want).abs() <= tol).all())
+    assert L.device_error() == 0

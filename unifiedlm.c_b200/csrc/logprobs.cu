@@ -586,12 +586,13 @@ bool lp_dtype_ok(int dt) { return dt == ULM_F32 || dt == ULM_BF16; }
 
 constexpr int LP_MAX_K_SPLITS = 32;
 
-// bf16 parts of the logits' gradient in bf16 precision. One part rounds each of its values by up to 2^-9
-// on the way to dh and dW, which with bf16 results makes their error 1.4 times that of the results' own
-// rounding (0.0024 against 0.0017), and up to twice that where few rows leave little to average (7 rows:
-// 0.0033). Two parts cost another pass of both products (V = 32000, D = 768: 81 -> 95 us for 256 rows, 100 ->
-// 140 for 512).
-int lp_parts(int64_t N) { return N <= 256 ? 2 : 1; }
+// bf16 parts of the logits' gradient in bf16 precision: two hold 16 of its digits (2^-17 of each value), so
+// that dh and dW have the error of their own rounding (0.0017 in bf16). One part rounds each value by up to
+// 2^-8 on the way (an error of 0.0024 to 0.0033, the more the fewer entries carry a row), and what rounding
+// adds to a row no longer sums to zero as the softmax's gradient does. The second part costs another pass of
+// both products and 2 bytes a logit (V = 32000, D = 768, backward: 512 rows 101 -> 140 us, 1024 142 -> 231,
+// 8192 920 -> 1705).
+constexpr int LP_PARTS = 2;
 constexpr int64_t LP_DUMP_BYTES = 256ll << 20;
 
 // How the head's forward finds the alternatives: from register lists of chunks where the rows are so many
@@ -617,8 +618,8 @@ int64_t lp_rows_at_once(int64_t N, int64_t V, int k) {
 // of 512 have 1e-6 and take 95 instead of 101 us there, 73 instead of 65 at 16 x 1416 x 768).
 //
 // A bf16 product whose 256 x 256 tiles fill the CTA pairs badly (8192 x 768: 96 tiles, two rounds of 74) is
-// split where the rounds saved are worth writing and adding the partial sums (that one over 32000: 346 us,
-// split in three 260 + 15).
+// split where the rounds saved are worth writing and adding the partial sums (one part of that one over
+// 32000: 346 us, split in three 260 + 15).
 int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
   int splits = 1;
   if (f32) {
@@ -626,8 +627,8 @@ int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
   } else {
     const int pairs = lp_sms() / 2;
     const int64_t tiles = cdiv(rows, 256) * cdiv(D, 256);
-    const double round_us = 2.0 * 256 * 256 * (double)k / 19e6;   // of all pairs, at 1400 TFLOP/s
-    const double part_us = (double)rows * (double)D * 8 / 6.5e6;  // a partial sum, written and read
+    const double round_us = 2.0 * 256 * 256 * (double)k * LP_PARTS / 19e6;  // of all pairs, at 1400 TFLOP/s
+    const double part_us = (double)rows * (double)D * 8 / 6.5e6;            // a partial sum, written and read
     double least = (double)cdiv(tiles, pairs) * round_us;
     for (int c = 2; c <= LP_MAX_K_SPLITS && c * 512 <= k; ++c) {
       const double t = (double)cdiv(tiles * c, pairs) / c * round_us + c * part_us + 5.0;
@@ -669,7 +670,7 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     w.w_parts = take(3 * V * ldd * 2);
   }
   if (backward) {
-    w.dx = take(N * ldv * (f32 ? 4 : 2 * lp_parts(N)));
+    w.dx = take(N * ldv * (f32 ? 4 : 2 * LP_PARTS));
     if (f32) w.dx_parts = take(3 * N * ldv * 2);
     // partial sums of dh, then of dW
     const int64_t room = lp_room(N, V);
@@ -824,7 +825,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   CUtensorMap th, tw, to;
   if (int rc = lp_operand(&th, h_op, ld_h, N, D, f32, w.h_parts, st)) return rc;
   if (int rc = lp_operand(&tw, w_op, ld_w, V, D, f32, w.w_parts, st)) return rc;
-  const int parts = f32 ? 1 : lp_parts(N);
+  const int parts = f32 ? 1 : LP_PARTS;
   ULM_REQUIRE(make_epi_tmap(&to, EPI_MODE_WARP, w.dx, f32 ? ULM_F32 : ULM_BF16, V, N, parts, ldv, N * ldv),
               "no tensor map of the logits' gradient");
   LpArgs a{};
@@ -833,7 +834,6 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   a.entropy = entropy;
   a.dlogprobs = dlogprobs;
   a.dentropy = dentropy;
-  a.parts = parts;
   if (int rc = f32 ? lp_launch<LP_GRAD, 0, true>(th, tw, to, s, a, st) : lp_launch<LP_GRAD, 0, false>(th, tw, to, s, a, st))
     return rc;
   const void *dx = w.dx, *hh = h_op, *ww = w_op;
@@ -847,7 +847,7 @@ extern "C" int ulm_lm_head_logprobs_bwd(const float* dlogprobs, const float* den
   // each product's operands are single matrices, or the parts of one (its batches)
   auto product = [&](const Operand& A, const Operand& B, int64_t rows, int64_t k, void* out, int dtype) -> int {
     GemmShape g{1, (int)rows, (int)D, (int)k, CAUSAL_NONE};
-    g.parts = f32 ? 6 : parts == 2 ? 2 : 0;
+    g.parts = f32 ? 6 : LP_PARTS;
     const int splits = lp_splits(rows, k, D, f32, lp_room(N, V));
     if (splits <= 1) return run_gemm(A, B, g, make_epilogue(EPI_STORE, dtype, out, D, rows * D, nullptr), st);
     g.batches = g.ksplit = splits;

@@ -10,8 +10,8 @@
 // k ln(chunks / k) times). LP_DUMP, for few rows, where most chunks of the short shares would enter, writes
 // all logits and the maxima of the chunks, and lp_join_kernel picks (2048 x 32000 x 768, k = 20: lists 191
 // us, written out 124; 16384 rows: 920 and 1140; no alternatives: 70 and 535, 1500 TFLOP/s).
-// LP_GRAD writes the logits' gradient ([v = t] a - p (a + b (log p + H))) in the operand type of the
-// products that follow.
+// LP_GRAD writes the logits' gradient ([v = t] a - p (a + b (log p + H))) for the products that follow: two
+// bf16 parts (hi and lo, the output map's batches), or fp32.
 //
 // Each CTA pair takes one run of consecutive tiles, all of the same length to within one, in an order
 // that keeps a row block until its columns are done: h's tile and the rows' state stay, W streams from
@@ -96,7 +96,6 @@ struct LpArgs {
   const float* entropy;
   const float* dlogprobs;
   const float* dentropy;
-  int parts;  // bf16 parts of the gradient: 1, or 2 (hi and lo, the output map's batches)
 };
 
 // The backward's factors of one row: dx_v = [v = t] a - p_v (a + b (log p_v + H)), with p_v = 2^l,
@@ -463,10 +462,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
         for (int i = 0; i < nch; ++i) {
           uint8_t* out = slots + (n % LPM_SLOTS) * 4096;
           ++n;
-          const bool two = !F32 && args.parts == 2;
           if (lane == 0) {
-            if (two)
-              bulk_wait_group_read<0>();  // both slots are taken
+            if (!F32)
+              bulk_wait_group_read<0>();  // the two parts take both slots
             else
               bulk_wait_group_read<LPM_SLOTS - 1>();  // the store before last has read its slot
           }
@@ -485,7 +483,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             }
             __syncwarp();
             stage_write<F32, 32>(out, lane, hh * (F32 ? 8 : 4), v);
-            if (two) {
+            if (!F32) {
 #pragma unroll
               for (int q = 0; q < 32; ++q) v[q] -= __bfloat162float(__float2bfloat16_rn(v[q]));
               stage_write<F32, 32>(slots + (n % LPM_SLOTS) * 4096, lane, hh * 4, v);
@@ -496,7 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
           if (lane == 0) {
             const int r0 = tile.rb * 256 + (int)rank * 128 + quad * 32;
             tma_store_3d(&tma_out, out, col_base + i * CW, r0, 0);
-            if (two) tma_store_3d(&tma_out, slots + (n % LPM_SLOTS) * 4096, col_base + i * CW, r0, 1);
+            if (!F32) tma_store_3d(&tma_out, slots + (n % LPM_SLOTS) * 4096, col_base + i * CW, r0, 1);
             bulk_commit_group();
           }
         }
