@@ -26,6 +26,19 @@ int stream_after(cudaStream_t to, cudaStream_t from);
 #include <cudaTypedefs.h>
 PFN_cuTensorMapEncodeTiled_v12000 encode_tiled();
 
+// f(), a call of that encoder. It wants a context that is current in the calling thread; a thread that has
+// done nothing on the GPU yet has none (one of autograd's whose buffers all came from the allocator's
+// cache), and the runtime's calls before it (cudaGetDevice) do not make one: cudaSetDevice does, also while
+// a stream is captured.
+template <typename F>
+CUresult encode_in_context(F&& f) {
+  CUresult r = f();
+  if (r != CUDA_ERROR_INVALID_CONTEXT) return r;
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || cudaSetDevice(d) != cudaSuccess) return r;
+  return f();
+}
+
 #define ULM_REQUIRE(cond, ...)                                  \
   do {                                                          \
     if (!(cond)) {                                              \

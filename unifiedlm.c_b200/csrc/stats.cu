@@ -1143,9 +1143,11 @@ inline int make_rows_tmap(CUtensorMap* map, const float* ptr, int64_t B, int64_t
   cuuint64_t strides[2] = {(cuuint64_t)M * 4, (cuuint64_t)(T * M) * 4};
   cuuint32_t box[3] = {32, (cuuint32_t)rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_in_context([&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled (scan tile) failed (%d)", (int)r);
     return ULM_ERR_CUDA;
