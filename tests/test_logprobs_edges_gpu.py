@@ -49,3 +49,32 @@ def test_head_backward_holds_the_logits_gradient_in_16_digits(N, V, D):
         tol = err + (n / 16 + 16) * 4 * U * mag + 1e-30
         assert bool(((got.double() - want).abs() <= tol).all())
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("k", [1, 2, 8, 9, 20])
+def test_alternatives_of_rows_whose_every_chunk_enters_the_list(k):
+    """Rows ascending from chunk to chunk of 32 logits: each chunk takes the place of the one that leaves,
+    with one alternative always the same place. Logits are exact (whole 1/1024s below 2^10): the
+    alternatives are the last ids, in the reverse order in descending rows."""
+    N, V, D = 9000, 32000, 64
+    v = torch.arange(V, device="cuda")
+    w = torch.zeros(V, D, device="cuda")
+    w[:, 0], w[:, 1], w[:, 2] = (v // 1024) * 4, (v // 32) % 32 / 8, (v % 32) / 1024
+    h = torch.zeros(N, D, device="cuda")
+    h[:, :3] = 1
+    h[1::3, :3] = -1
+    h[2::3, :3] = 0.5
+    t = torch.arange(N, device="cuda") % V
+    w, h = w.bfloat16(), h.bfloat16()
+    x = h[:3, :3].double() @ w[:, :3].double().t()
+    logp = torch.log_softmax(x, -1)
+    for _ in range(3):
+        r = lm_head_logprobs(h, w, t, top_k=k)
+        for i in range(3):
+            ids = torch.arange(k, device="cuda") if i == 1 else V - 1 - torch.arange(k, device="cuda")
+            assert bool((r.top_ids[i::3] == ids).all())
+            want = logp[i, ids]
+            # log s of 32000 powers: each off by 2^-22 and by its argument's rounding (up to 160 log2 e)
+            tol = (V / 32 + 32) * U + 2.0 ** -22 + 320 * U + 4 * U * 160
+            assert bool(((r.top_logprobs[i::3].double() - want).abs() <= tol).all())
+    assert L.device_error() == 0

@@ -177,7 +177,9 @@ struct LpRun {
           v[0] = lm;
           id[0] = mine;
         }
-        bulk_wait_group_read<0>();  // the chunk before has left the stage
+        // the chunk before has left the stage and has landed: it may be the one whose place is taken now, and
+        // two copies in flight to one address have no order
+        bulk_wait_group<0>();
         float4* d = reinterpret_cast<float4*>(stage);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
