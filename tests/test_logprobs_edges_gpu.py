@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import unifiedlm_c_b200._lib as L
-from unifiedlm_c_b200.logprobs import lm_head_logprobs
+from unifiedlm_c_b200.logprobs import lm_head_logprobs, token_logprobs
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -77,4 +77,30 @@ def test_alternatives_of_rows_whose_every_chunk_enters_the_list(k):
             # log s of 32000 powers: each off by 2^-22 and by its argument's rounding (up to 160 log2 e)
             tol = (V / 32 + 32) * U + 2.0 ** -22 + 320 * U + 4 * U * 160
             assert bool(((r.top_logprobs[i::3].double() - want).abs() <= tol).all())
+    assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("N,V", [(1, 32000), (3, 16384), (37, 33001), (80, 20000)])
+def test_rows_split_over_a_cluster_again_and_again(N, V):
+    """Few rows: a row's CTAs store their results into the first one's shared memory. Many calls one after
+    another, on two streams beside a product that keeps the GPU full: the same bits each time."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(N, V, device="cuda", generator=gen) * 3
+    t = torch.randint(0, V, (N,), device="cuda", generator=gen)
+    big = torch.randn(4096, 4096, device="cuda", generator=gen).bfloat16()
+    want = [o.clone() for o in token_logprobs(x, t, top_k=9)]
+    logp = torch.log_softmax(x.double(), -1)
+    assert torch.equal(want[2], torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :9])
+    rs = (V / 32 + 32) * U + 2.0 ** -22 + 80 * U
+    assert bool(((want[0] - logp.gather(1, t[:, None])[:, 0]).abs() <= rs + 4 * U * 40).all())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for i in range(60):
+        with torch.cuda.stream(streams[i % 2]):
+            if i % 10 == 0:
+                big @ big
+            got.append(token_logprobs(x, t, top_k=9))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
     assert L.device_error() == 0

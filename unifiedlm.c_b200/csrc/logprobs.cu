@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   __shared__ uint64_t cand[LP_CAP];
   __shared__ uint64_t red[LP_THREADS / 32];
   __shared__ int count;
+  if (split > 1) cluster_arrive_relaxed();  // this CTA has started; waited for before the first remote store
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
   const int rank = split > 1 ? (int)cluster_ctarank() : 0;
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   }
   if (lane == 0) wsum[wp] = make_float2(st.s, st.u);
   __syncthreads();
+  if (split > 1) cluster_wait_acquire();  // the first CTA's shared memory is there
   if (tid == 0) {
     LpStat all{st.m, st.m2, 0.f, 0.f};
 #pragma unroll
