@@ -6,6 +6,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libulm_b200.so")
@@ -145,15 +146,35 @@ def device_error():
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
+_C = torch._C
+_PRE_DISPATCH = _C.DispatchKey.PreDispatch
+
+
+def _observed():
+    """Whether something looks on at the dispatcher's calls or transforms them: a dispatch mode (make_fx, a
+    FLOP counter, selective checkpointing), torch.jit.trace, a torch.func transform, an open level of
+    forward-mode differentiation."""
+    return (_C._len_torch_dispatch_stack() > 0 or _C._get_tracing_state() is not None or
+            _C._are_functorch_transforms_active() or forward_ad._current_level >= 0 or
+            _C._dispatch_tls_is_dispatch_key_included(_PRE_DISPATCH))
+
+
 def eager(*ts):
-    """Whether the tensors hold data that a call can read now (nothing is traced, compiled or faked): the
-    entries then call the library directly, without the dispatcher's cost of a custom op."""
-    if torch.compiler.is_compiling():
+    """Whether the tensors hold data that a call can read now and nobody else is to see the call (nothing is
+    traced, compiled, faked, transformed or observed): the entries then call the library directly, without
+    the dispatcher's cost of a custom op."""
+    if torch.compiler.is_compiling() or _observed():
         return False
     for t in ts:
         if type(t) not in _PLAIN:
             return False
     return True
+
+
+def no_tangents(name, *ts):
+    """Refuses inputs that carry a tangent (forward-mode differentiation), which the call would drop."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def first_order(name):

@@ -119,6 +119,7 @@ def embedding(tokens, weight, scale=1.0, out_dtype=None):
     tk = tk.to(torch.int64).contiguous()
     args = tk, w, float(scale), out_dtype == torch.bfloat16
     if not L.eager(tk, w):
+        L.no_tangents("embedding", w)
         y = torch.ops.ulm.embedding_fwd(*args)
     elif w.requires_grad and torch.is_grad_enabled():
         y = _Embedding.apply(*args)

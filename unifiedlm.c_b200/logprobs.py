@@ -308,6 +308,7 @@ def lm_head_logprobs(h, weight, tokens, top_k=0, precision="bf16"):
     ww = weight if weight.dtype in (torch.float32, torch.bfloat16) else weight.float()
     args = hh, ww, _rows(tokens), top_k, PRECISION[precision]
     if not L.eager(hh, ww, tokens):
+        L.no_tangents("lm_head_logprobs", hh, ww)
         out = torch.ops.ulm.lm_head_logprobs_fwd(*args)
     elif (hh.requires_grad or ww.requires_grad) and torch.is_grad_enabled():
         out = _HeadLogprobs.apply(*args)
@@ -325,6 +326,7 @@ def token_logprobs(logits, tokens, top_k=0):
         x = x.contiguous()
     tk = _rows(tokens)
     if not L.eager(x, tokens):
+        L.no_tangents("token_logprobs", x)
         out = torch.ops.ulm.token_logprobs_fwd(x, tk, top_k)
     elif x.requires_grad and torch.is_grad_enabled():
         out = _TokenLogprobs.apply(x, tk, top_k)
