@@ -6,6 +6,7 @@ import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
+from unifiedlm_c_b200.clip import clip_grads, grad_norm
 from unifiedlm_c_b200.embed import embedding
 from unifiedlm_c_b200.logprobs import lm_head_logprobs, token_logprobs
 
@@ -76,3 +77,28 @@ def test_forward_mode_is_refused(name):
         torch.func.jvp(f, (a,), (b,))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda x: f(x)[0].sum())(a)
+
+
+def test_clipping_is_not_traced():
+    w, _, a, b = inputs()
+    calls = (lambda x: grad_norm([x]), lambda x: clip_grads([x], 1.0, out=[w[:20]]), lambda x: clip_grads([x], 1.0))
+    for f in calls:
+        before = a.clone()
+        for way in (lambda: make_fx(f)(a), lambda: make_fx(f, pre_dispatch=True)(a), lambda: torch.jit.trace(f, (a,)),
+                    lambda: torch.func.vmap(f)(torch.stack([a, b]))):
+            with pytest.raises(RuntimeError, match="traced"):
+                way()
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(forward_ad.make_dual(a, b))
+        assert torch.equal(a, before)
+
+
+def test_clipping_where_something_looks_on():
+    """A dispatch mode that records nothing, and torch.compile, which breaks its graph at the call."""
+    _, _, a, _ = inputs()
+    want = clip_grads([a], 1.0, out=[torch.empty_like(a)])
+    with Seen():
+        assert torch.equal(clip_grads([a], 1.0, out=[torch.empty_like(a)]), want)
+    f = torch.compile(lambda x: clip_grads([x * 1.0], 1.0), backend="eager")
+    assert torch.equal(f(a), want)

@@ -177,6 +177,20 @@ def no_tangents(name, *ts):
         raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
+_PROXY = _C._TorchDispatchModeKey.PROXY
+
+
+def not_traced(name, ts):
+    """Refuses a call that is no op of the dispatcher where something would record it, or transform its
+    inputs: the record would lack it."""
+    if not _observed():
+        return
+    if (_C._get_tracing_state() is not None or _C._get_dispatch_mode(_PROXY) is not None or
+            _C._dispatch_tls_is_dispatch_key_included(_PRE_DISPATCH) or _C._are_functorch_transforms_active()):
+        raise RuntimeError(f"{name} cannot be traced or transformed")
+    no_tangents(name, *ts)
+
+
 def first_order(name):
     """Called in a backward: refuses the one that is to be differentiated again (create_graph)."""
     if torch.is_grad_enabled():

@@ -7,7 +7,8 @@ takes parameters, `clip_grads` a list of gradients (in place, or into other tens
 as `GradBucket`'s views), `grad_norm` only measures. Squares are added in fp64 in a fixed order, so
 the norm is the same in every run. A norm that is not finite makes the factor what IEEE division
 gives (0 or NaN), as torch's function does. The work runs in libulm_b200.so (ulm_clip_grads) on the
-current stream. No CPU path.
+current stream. No CPU path. Tracers (make_fx, torch.jit.trace) and gradients with a tangent are refused;
+torch.compile breaks its graph at the call.
 """
 import math
 from array import array
@@ -28,6 +29,8 @@ def _codes(ts):
 
 
 def _run(grads, outs, max_norm):
+    if not torch.compiler.is_compiling():
+        L.not_traced("gradient clipping", grads)
     at = grads[0].get_device()
     for g in grads:
         if g.get_device() != at or at < 0:
@@ -63,10 +66,11 @@ def _run(grads, outs, max_norm):
 
 def grad_norm(grads):
     """The 2-norm over all tensors of `grads` (fp32 or bf16, one GPU), a 0-d fp32 tensor."""
-    grads = [g.detach() for g in grads if g is not None]
+    grads = [g for g in grads if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    return _run(grads, None, 0.0)
+    with torch.no_grad():
+        return _run(grads, None, 0.0)
 
 
 def clip_grads(grads, max_norm, out=None):
