@@ -461,7 +461,8 @@ int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const 
                            int64_t N, int64_t V, void* stream);
 
 /* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd.
- * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 16-byte aligned. */
+ * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 16-byte aligned; the function is
+ * called with the device of the launch current (its SMs are part of the size). */
 int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens,
                              float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
                              void* work, int64_t N, int64_t V, int64_t D, int top_k, int prec, void* stream);

@@ -71,8 +71,9 @@ def lm_head_logprobs_fwd_raw(h, weight, tokens, top_k, precision, stats=True):
     opt = _op_dtype(precision)
     h_op, ld_h = _operand(h, opt)
     w_op, ld_w = _operand(weight, opt)
-    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, top_k, 0, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
+        work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, top_k, 0, precision), device=h.device,
+                           dtype=torch.uint8)
         L.check(lib.ulm_lm_head_logprobs_fwd(h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(),
                                              lp.data_ptr(), ent.data_ptr(), _addr(st), ids.data_ptr(), tlp.data_ptr(),
                                              work.data_ptr(), N, V, D, top_k, precision, L.stream(h.device)))
@@ -89,8 +90,9 @@ def lm_head_logprobs_bwd_raw(dlp, dent, h, weight, tokens, stats, ent, precision
     opt = _op_dtype(precision)
     h_op, ld_h = _operand(h, opt)
     w_op, ld_w = _operand(weight, opt)
-    work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, 1, precision), device=h.device, dtype=torch.uint8)
     with L.on(h.device):
+        work = torch.empty(lib.ulm_lm_head_logprobs_work_bytes(N, V, D, 0, 1, precision), device=h.device,
+                           dtype=torch.uint8)
         L.check(lib.ulm_lm_head_logprobs_bwd(
             _addr(dlp), _addr(dent), h_op.data_ptr(), ld_h, w_op.data_ptr(), ld_w, tokens.data_ptr(), stats.data_ptr(),
             ent.data_ptr(), _addr(dh), L.dtype_code(h.dtype), _addr(dw), L.dtype_code(weight.dtype), work.data_ptr(),
