@@ -460,7 +460,9 @@ int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const 
                            const int64_t* tokens, const float* stats, const float* entropy, void* dlogits, int64_t ld_d,
                            int64_t N, int64_t V, void* stream);
 
-/* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd.
+/* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd. Logits
+ * are finite here, not masks: a row with a NaN or +inf among its products has NaN results, one with -inf a NaN entropy (and NaN gradients of it); the top_ids of
+ * such rows are top_k different tokens.
  * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 16-byte aligned; the function is
  * called with the device of the launch current (its SMs are part of the size). */
 int ulm_lm_head_logprobs_fwd(const void* h_op, int64_t ld_h, const void* w_op, int64_t ld_w, const int64_t* tokens,

@@ -104,3 +104,18 @@ def test_rows_split_over_a_cluster_again_and_again(N, V):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("N,V,k,bad", [(3, 40, 32, 20), (3, 40, 32, 39), (300, 500, 20, 7), (9000, 8000, 8, 300), (9000, 8000, 1, 2)])
+def test_alternatives_of_rows_with_some_nan(N, V, k, bad):
+    """Weight rows of NaN: every row of logits holds some. NaN results, and k different tokens as
+    alternatives."""
+    h, w, t, gen = on_grid(N, V, 64, N, torch.bfloat16)
+    w[torch.randperm(V, device="cuda", generator=gen)[:bad]] = float("nan")
+    r = lm_head_logprobs(h, w, t, top_k=k)
+    assert bool(r.logprobs[t >= 0].isnan().all()) and bool((r.logprobs[t < 0] == 0).all())
+    assert bool(r.entropy.isnan().all()) and bool(r.top_logprobs.isnan().all())
+    assert bool((r.top_ids >= 0).all()) and bool((r.top_ids < V).all())
+    ids = r.top_ids.sort(-1).values
+    assert bool((ids[:, 1:] != ids[:, :-1]).all())
+    assert L.device_error() == 0

@@ -770,10 +770,20 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
     top_ids[row * k + r] = lp_key_id(key[c]);
     top_logprobs[row * k + r] = (lp_key_value(key[c]) - m) - logs;
   });
-  // only a row with NaN among its logits has fewer than k others
-  if (tid >= n && tid < k) {
-    top_ids[row * k + tid] = tid;
-    top_logprobs[row * k + tid] = __uint_as_float(0x7FC00000u);
+  // Only a row with NaN or -inf among its logits has fewer than k others: the lowest ids that are not there yet
+  // (of the first k at least k - n are free) take the places left.
+  if (n < k && tid < k) {
+    auto taken = [&](uint32_t id) {
+      for (int j = 0; j < n; ++j)
+        if (lp_key_id(key[j]) == id) return true;
+      return false;
+    };
+    int place = n;
+    for (int c = 0; c < tid; ++c) place += taken((uint32_t)c) ? 0 : 1;
+    if (place < k && !taken((uint32_t)tid)) {
+      top_ids[row * k + place] = tid;
+      top_logprobs[row * k + place] = __uint_as_float(0x7FC00000u);
+    }
   }
 }
 constexpr int LP_MAX_GROUPS = 128;

@@ -11,8 +11,10 @@ and the `top_k` best tokens in descending order (the lower id first among equals
 `head.lm_head_loss`; `token_logprobs(logits, tokens)` takes logits that exist already (a decode
 step's, `BatchedDecoder.logprobs`). Both are differentiable in logprobs and entropy. Token -1 is
 padding: logprob 0, no gradient through it. Any other token outside the vocabulary makes its
-logprob, and the gradients that it reaches, NaN. Masked tokens (logits of -inf) have probability 0;
-a row that is masked throughout, or holds a NaN or +inf, has NaN results, as log_softmax has. The
+logprob, and the gradients that it reaches, NaN. Masked tokens (logits of -inf) of `token_logprobs`
+have probability 0; a row that is masked throughout, or holds a NaN or +inf, has NaN results, as
+log_softmax has. The products of `lm_head_logprobs` are taken as finite: a row with one that is not has
+a NaN entropy (and logprobs, but for -inf), and its alternatives are some top_k different tokens. The
 work runs in libulm_b200.so (ulm_lm_head_logprobs_*, ulm_token_logprobs_*) through `torch.library`
 ops. No CPU path.
 """
