@@ -461,7 +461,8 @@ int ulm_token_logprobs_bwd(const float* dlogprobs, const float* dentropy, const 
                            int64_t N, int64_t V, void* stream);
 
 /* The same of the logits x = h W^T: h_op (N, ld_h) and w_op (V, ld_w) as for ulm_lm_head_loss_fwd. Logits
- * are finite here, not masks: a row with a NaN or +inf among its products has NaN results, one with -inf a NaN entropy (and NaN gradients of it); the top_ids of
+ * are finite here, not masks: a row with a NaN or +inf among its products, below -1e30 throughout, or with
+ * one past 2.3e38, has NaN results, one with -inf a NaN entropy (and NaN gradients of it); the top_ids of
  * such rows are top_k different tokens.
  * work: ulm_lm_head_logprobs_work_bytes(N,V,D,top_k,0,prec) bytes, 16-byte aligned; the function is
  * called with the device of the launch current (its SMs are part of the size). */

@@ -119,3 +119,25 @@ def test_alternatives_of_rows_with_some_nan(N, V, k, bad):
     ids = r.top_ids.sort(-1).values
     assert bool((ids[:, 1:] != ids[:, :-1]).all())
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("N,V,k", [(5, 300, 4), (9000, 8000, 8)])
+def test_head_rows_past_the_range(N, V, k):
+    """Products below -1e30 throughout, or beyond 2.3e38: NaN, not an infinite or a finite answer; other rows
+    as they are."""
+    h, w, t, _ = on_grid(N, V, 64, 1, torch.bfloat16)
+    t = t.clamp(min=0)
+    h[:, 0], w[:, 0] = 0, 2.0 ** 60
+    want = lm_head_logprobs(h, w, t, top_k=k)
+    h[1, 0], h[3, 0] = -(2.0 ** 50), 2.0 ** 67 * 1.75  # -1.3e33 and 3e38
+    r = lm_head_logprobs(h, w, t, top_k=k)
+    for i in (1, 3):
+        assert bool(r.logprobs[i].isnan()) and bool(r.entropy[i].isnan()) and bool(r.top_logprobs[i].isnan().all())
+        ids = r.top_ids[i].sort().values
+        assert bool((ids[1:] != ids[:-1]).all()) and 0 <= int(ids[0]) and int(ids[-1]) < V
+    keep = (torch.arange(N, device="cuda") != 1) & (torch.arange(N, device="cuda") != 3)
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(r, want))
+    hh, ww = h.requires_grad_(), w.requires_grad_()
+    r = lm_head_logprobs(hh, ww, t)
+    dh, = torch.autograd.grad(r.logprobs.sum(), hh)
+    assert bool(dh[1].isnan().all()) and bool(dh[3].isnan().all()) and bool(dh[keep].isfinite().all())

@@ -158,7 +158,7 @@ struct LpRun {
   __device__ __forceinline__ void add(float (&x)[32], int col0, int V, float* dump, uint8_t* stage) {
     if (col0 + 32 > V) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = col0 + i < V ? x[i] : -1e30f;
+      for (int i = 0; i < 32; ++i) x[i] = col0 + i < V ? x[i] : -1e35f;  // no power, in any row
     }
     float lm = fmaxf(x[0], x[1]);
 #pragma unroll
@@ -624,8 +624,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 32 * LP_JOIN_ROWS : TPR)
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) merge(wred[i].x, wred[i].y, wred[i].z);
   }
-  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e
-  const float logs = logf(s) + fmaf(-m, LOG2E, m2) * LN2;
+  // logp = (x - m) - logs: log s, and how far m2 is from m log2 e. No power is left of a row below -1e30
+  // throughout, or past 2.3e38: NaN.
+  const float logs = s > 0.f ? logf(s) + fmaf(-m, LOG2E, m2) * LN2 : __uint_as_float(0x7FC00000u);
   if (tid == 0) {
     const int64_t t = args.tokens[row];
     logprobs[row] = t == -1 ? 0.f : t < 0 || t >= shape.V ? __uint_as_float(0x7FC00000u) : (args.given[row] - m) - logs;
