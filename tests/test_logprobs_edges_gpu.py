@@ -141,3 +141,21 @@ def test_head_rows_past_the_range(N, V, k):
     r = lm_head_logprobs(hh, ww, t)
     dh, = torch.autograd.grad(r.logprobs.sum(), hh)
     assert bool(dh[1].isnan().all()) and bool(dh[3].isnan().all()) and bool(dh[keep].isfinite().all())
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp32"])
+def test_the_entropys_gradient_does_not_see_the_token(precision):
+    """A token out of range makes its logprob NaN, and the gradients through it; the entropy and its
+    gradient have nothing of it."""
+    dtype = torch.bfloat16 if precision == "bf16" else torch.float32
+    h, w, t, _ = on_grid(7, 300, 64, 2, dtype)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    x = (torch.randn(7, 300, device="cuda") * 2).to(dtype).requires_grad_()
+    bad = t.clone()
+    bad[1], bad[4] = 300, -5
+    for call, leaves in ((lambda t: lm_head_logprobs(h, w, t, precision=precision), [h, w]), (lambda t: token_logprobs(x, t), [x])):
+        want = torch.autograd.grad(call(t).entropy.sum(), leaves)
+        got = torch.autograd.grad(call(bad).entropy.sum(), leaves)
+        assert all(torch.equal(a, b) and bool(a.isfinite().all()) for a, b in zip(got, want))
+        through = torch.autograd.grad(call(bad).logprobs.sum(), leaves)
+        assert all(bool(g.isnan().any()) for g in through)

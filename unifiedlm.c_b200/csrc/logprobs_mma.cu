@@ -125,7 +125,7 @@ __device__ __forceinline__ LpCoef lp_coef(const int64_t* tokens, const float* st
   c.m = stats[2 * r];
   c.l2 = stats[2 * r + 1] * LOG2E;
   c.a = c.t == -1 || !dlogprobs ? 0.f : dlogprobs[r];
-  if (c.t < -1 || c.t >= V) c.a = __uint_as_float(0x7FC00000u);
+  if (dlogprobs && (c.t < -1 || c.t >= V)) c.a = __uint_as_float(0x7FC00000u);  // (the entropy does not see t)
   const float b = dentropy ? dentropy[r] : 0.f;
   c.b2 = b * LN2;
   c.c0 = c.a + (b != 0.f ? b * entropy[r] : 0.f);
