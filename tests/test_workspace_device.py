@@ -39,3 +39,18 @@ def test_work_buffer_is_sized_on_the_operands_device(monkeypatch, backward):
     else:
         lm_head_logprobs_fwd_raw(h, w, t, 2, L.ULM_PREC_BF16)
     assert len(lib.seen) == 2 and all(inside for _, inside in lib.seen)
+
+
+def test_work_buffer_holds_what_the_backward_writes():
+    """Two bf16 parts of the logits' gradient, and partial sums only where a product is split; in fp32
+    precision the gradient, its three parts, the operands' parts and 64 MB for sums."""
+    size = L.lib().ulm_lm_head_logprobs_work_bytes
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    for N, V, D in ((1, 64, 32), (256, 512, 1024), (300, 505, 200)):
+        ldv, ldd = (V + 7) // 8 * 8, (D + 7) // 8 * 8
+        assert size(N, V, D, 0, 1, L.ULM_PREC_BF16) == up(N * ldv * 4)
+        f32 = size(N, V, D, 0, 1, L.ULM_PREC_FP32)
+        least = up(N * ldv * 4) + up(N * ldv * 6) + up(N * ldd * 6) + up(V * ldd * 6)
+        assert least <= f32 <= least + (64 << 20)
+    N, V, D = 8192, 32000, 768  # dh in three ranges of the vocabulary, dW whole
+    assert size(N, V, D, 0, 1, L.ULM_PREC_BF16) == N * V * 4 + 3 * N * D * 4

@@ -643,6 +643,12 @@ int lp_splits(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
   return splits > 1 ? (int)cdiv(k, ksplit_chunk((int)k, splits)) : 1;  // no empty range
 }
 
+// Rows of partial sums of that product: none where it is not split.
+int64_t lp_sum_rows(int64_t rows, int64_t k, int64_t D, bool f32, int64_t room) {
+  const int splits = lp_splits(rows, k, D, f32, room);
+  return splits > 1 ? splits * rows : 0;
+}
+
 // Floats for an fp32 product's sums: 64 MB of them, or the place of the fp32 gradient of the logits, which
 // its parts have replaced by then, where that is larger (that place alone would hold too few of them where the
 // vocabulary is little wider than the model: 16 x 1416 x 768 107 us and an error of 2.7e-6, now 65 and 5e-7;
@@ -679,7 +685,7 @@ LpWork lp_work(void* base, int64_t N, int64_t V, int64_t D, int k, bool backward
     if (f32 && room > LP_SUMS)
       w.sums = static_cast<float*>(w.dx);
     else
-      w.sums = floats(std::max(lp_splits(N, V, D, f32, room) * N, lp_splits(V, N, D, f32, room) * V) * D);
+      w.sums = floats(std::max(lp_sum_rows(N, V, D, f32, room), lp_sum_rows(V, N, D, f32, room)) * D);
   } else {
     const int64_t rows = lp_rows_at_once(N, V, k);
     // the shares of the rows of one launch: all of them, but for the last one's fewer rows
