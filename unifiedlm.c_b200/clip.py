@@ -28,6 +28,76 @@ def _codes(ts):
         raise L.UlmError(f"unsupported element type {e.args[0]}") from None
 
 
+def _dims(t):
+    """{stride: size} of a tensor in bytes, its elements the innermost dimension; None where two of its
+    dimensions have the same stride."""
+    es = t.element_size()
+    dims = {1: es}
+    for n, s in zip(t.shape, t.stride()):
+        if n > 1 and s > 0:
+            if s * es in dims:
+                return None
+            dims[s * es] = n
+    return dims
+
+
+def _folded(t):
+    """Whether elements of a tensor share memory (or may: each stride is to pass what lies within it)."""
+    inner = 0
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s <= inner:
+            return True
+        inner += (n - 1) * s
+    return False
+
+
+def _end(t):
+    return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _apart(a, b):
+    """Whether two tensors have no byte in common. Written in the strides of both, every address is one row
+    of digits, as long as no digit of either tensor runs over into the next: they are apart where one
+    digit's ranges are. Two starts to count from are tried; what cannot be written so is not apart."""
+    if _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr():
+        return True
+    da, db = _dims(a), _dims(b)
+    if da is None or db is None:
+        return False
+    strides = sorted({*da, *db}, reverse=True)
+    for base in (min(a.data_ptr(), b.data_ptr()), a.untyped_storage().data_ptr()):
+        ranges, exact = [], True
+        for t, d in ((a, da), (b, db)):
+            at, digits, last = t.data_ptr() - base, [], 0
+            for s in strides:
+                low, at = divmod(at, s)
+                digits.append((low, low + d.get(s, 1) - 1))
+            for s, outer, (_, high) in zip(strides[:0:-1], strides[-2::-1], digits[:0:-1]):
+                last += high * s
+                exact = exact and last < outer
+            ranges.append(digits)
+        if exact:
+            return any(x[1] < y[0] or y[1] < x[0] for x, y in zip(*ranges))
+    return False
+
+
+def _check_strided(grads, outs):
+    """The library's refusals of overlaps, for lists with tensors that it gets as copies."""
+    if any(_folded(o) for o in outs):
+        raise ValueError("an output whose elements share memory")
+    items = [(o.data_ptr(), _end(o), i, True, o) for i, o in enumerate(outs) if o.numel()]
+    if outs is not grads:
+        items += [(g.data_ptr(), _end(g), i, False, g) for i, (g, o) in enumerate(zip(grads, outs)) if g.numel() and g is not o]
+    items.sort(key=lambda x: x[:2])
+    reach = []  # those that go on past the one at hand
+    for x in items:
+        reach = [y for y in reach if y[1] > x[0]]
+        for y in reach:
+            if (x[3] or y[3]) and x[2] != y[2] and not _apart(x[4], y[4]):
+                raise L.UlmError(f"gradient {x[2]} overlaps another one's output (the same tensor twice?)")
+        reach.append(x)
+
+
 def _run(grads, outs, max_norm):
     if not torch.compiler.is_compiling():
         L.not_traced("gradient clipping", grads)
@@ -40,13 +110,19 @@ def _run(grads, outs, max_norm):
         if g.layout is not torch.strided:
             raise ValueError("sparse gradients are not supported")
     n = len(grads)
-    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    plain = [g.is_contiguous() for g in grads]
+    src = grads if all(plain) else [g if c else g.contiguous() for g, c in zip(grads, plain)]
     dst = None
     if outs is grads:
         dst = src
+        if src is not grads:
+            _check_strided(grads, outs)
     elif outs is not None:
-        dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
-               for g, s, o in zip(grads, src, outs)]
+        plain_out = [o.is_contiguous() for o in outs]
+        if src is not grads or not all(plain_out):
+            _check_strided(grads, outs)
+        dst = [s if o is g else o if c else torch.empty_like(o, memory_format=torch.contiguous_format)
+               for g, s, o, c in zip(grads, src, outs, plain_out)]
     lib, dev = L.lib(), grads[0].device
     norm = torch.empty((), device=dev, dtype=torch.float32)
     work = torch.empty(lib.ulm_clip_grads_work_bytes(n), device=dev, dtype=torch.uint8)
@@ -77,7 +153,7 @@ def clip_grads(grads, max_norm, out=None):
     """Scales `grads` (fp32 or bf16 tensors of one GPU) to a 2-norm of at most `max_norm`, in place, or
     into the tensors `out` of the same shapes (fp32 or bf16 each). Returns the norm that they had, a 0-d
     fp32 tensor. A tensor may stand in the list once: one that is there twice, or overlaps another, is
-    refused."""
+    refused, before anything is written."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
