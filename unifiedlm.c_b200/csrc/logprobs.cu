@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   __shared__ float wmax[LP_THREADS / 32];
   __shared__ float2 wsum[LP_THREADS / 32];
   __shared__ alignas(16) LpStat runs[LP_MAX_SPLIT];                    // of the cluster's CTAs (first CTA)
-  __shared__ uint64_t best[LP_MAX_SPLIT * LP_MAX_TOP];     // their alternatives, 0 for none (first CTA)
+  __shared__ uint64_t best[LP_MAX_SPLIT * LP_MAX_TOP];     // their alternatives (first CTA)
   __shared__ alignas(16) float gmax[LP_GROUPS];
   __shared__ float kept[LP_KEPT * LP_THREADS];
   __shared__ float thr_s;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
     __syncthreads();
     const int n = count;
     if (n <= LP_CAP && (n >= k || !few)) {
-      // each candidate's place is the number of better ones
+      // each candidate's place is the number of better ones (above a threshold there are k at least)
       for (int c = tid; c < n; c += LP_THREADS) {
         const uint64_t key = cand[c];
         int place = 0;
@@ -354,7 +354,6 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
         for (int j = 0; j < n; ++j) place += cand[j] > key ? 1 : 0;
         if (place < k) give(place, key);
       }
-      if (n + tid < k) give(n + tid, 0);
     } else {
       // more equal logits than the list holds, or too few that are not masked: the best one after the
       // last, k times
@@ -424,7 +423,6 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS<T>)
   const int n = split * k;
   for (int c = tid; c < n; c += LP_THREADS) {
     const uint64_t key = best[c];
-    if (key == 0) continue;
     int place = 0;
     for (int j = 0; j < n; ++j) place += best[j] > key ? 1 : 0;
     if (place < k) {
