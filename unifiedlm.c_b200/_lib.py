@@ -215,4 +215,4 @@ _HERE = _Here()
 
 def on(device):
     """`torch.cuda.device(device)`, or nothing where it is the current one already."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _C._cuda_getDevice() == device.index else torch.cuda.device(device)
