@@ -67,10 +67,10 @@ __device__ __forceinline__ LpTile lp_tile(const LpShape& s, int64_t t) {
   const int64_t per_group = (int64_t)s.group * s.row_blocks;
   LpTile r;
   r.g = (int)(t / per_group);
-  const int rem = (int)(t - r.g * per_group);
+  const int64_t rem = t - r.g * per_group;  // 2^28 rows and more of a wide vocabulary pass 32 bits
   const int wide = min(s.group, s.col_tiles - r.g * s.group);
-  r.rb = rem / wide;
-  r.ct = r.g * s.group + rem - r.rb * wide;
+  r.rb = (int)(rem / wide);
+  r.ct = r.g * s.group + (int)(rem - (int64_t)r.rb * wide);
   return r;
 }
 
