@@ -60,7 +60,7 @@ struct GemmShape {
   // > 0: operands in bf16 parts (hi first), which are their batches (one output batch, or one for each
   // range of ksplit); the k range is walked once for each pair of parts, the small products first.
   // 6: fp32 operands, three parts each (hi, mid, lo), pairs GEMM_PART_A / GEMM_PART_B; left out are the
-  // products below 2^-25 of the whole one. 2: A has two parts, B is whole.
+  // products of a second and a third part or less, up to 2^-24 of the whole one. 2: A has two parts, B is whole.
   // B is MN-major.
   int parts = 0;
 };

@@ -1,6 +1,7 @@
-// The products x = h W^T of the log-probability entries, whose logits never leave the SM: a tcgen05
-// kernel on CTA pairs (256 x 256 tiles, cta_group::2, operands by TMA, accumulators double-buffered in
-// tensor memory) with two epilogues.
+// The products x = h W^T of the log-probability entries: a tcgen05 kernel on CTA pairs (256 x 256 tiles,
+// cta_group::2, operands by TMA, accumulators double-buffered in tensor memory) with three epilogues. The
+// logits stay on the SM where no alternatives are asked for; with lists, the chunks of 32 that enter one
+// leave it, and LP_DUMP writes them all.
 //
 // LP_STATS keeps, for each row, the running maximum, sum of exponentials and entropy sum of the softmax in
 // registers from tile to tile; an epilogue thread owns half of a row's columns, in chunks of 32 logits.
@@ -20,8 +21,8 @@
 // looking through the k best chunks of each row.
 //
 // fp32 operands are given as three bf16 parts each (x = hi + mid + lo to the last bit, lp_split_kernel),
-// and the product runs over six pairs of parts, the small ones first: what is left out is below 2^-25 of
-// each product. Bound by the tensor cores either way.
+// and the product runs over six pairs of parts, the small ones first: what is left out is up to 2^-24
+// of each product (two pairs of a second and a third part). Bound by the tensor cores either way.
 #include <algorithm>
 
 #include "gemm.cuh"
