@@ -88,3 +88,9 @@ def test_expanded_gradients_into_other_tensors():
     _check_strided([row, a[:, 4:8]], [torch.zeros(8, 4), a[:, 8:]])
     with pytest.raises(L.UlmError, match="overlap"):
         _check_strided([row, a[:, 4:8]], [torch.zeros(8, 4), a[:, :4]])
+
+
+def test_apart_of_expanded_rows():
+    a = torch.zeros(8, 12)
+    x, y = a[:1, :4].expand(8, 4), a[:1, 3:7].expand(8, 4)
+    assert not _apart(x, y) and _apart(x, a[:1, 4:8].expand(8, 4))

@@ -52,6 +52,8 @@ def _folded(t):
 
 
 def _end(t):
+    if t.is_contiguous():
+        return t.data_ptr() + t.nbytes
     return t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
@@ -61,6 +63,13 @@ def _apart(a, b):
     digit's ranges are. Two starts to count from are tried; what cannot be written so is not apart."""
     if _end(a) <= b.data_ptr() or _end(b) <= a.data_ptr():
         return True
+    if a.dim() == 2 and a.stride() == b.stride() and a.stride(1) == 1 and a.stride(0) > 0 and a.dtype == b.dtype:
+        # blocks of one matrix (slices of a fused gradient): the digits below, its rows and columns
+        base, es, pitch = a.untyped_storage().data_ptr(), a.element_size(), a.stride(0)
+        (ra, ca), (rb, cb) = (divmod((t.data_ptr() - base) // es, pitch) for t in (a, b))
+        (na, wa), (nb, wb) = a.shape, b.shape
+        if ca + wa <= pitch and cb + wb <= pitch:
+            return ra + na <= rb or rb + nb <= ra or ca + wa <= cb or cb + wb <= ca
     da, db = _dims(a), _dims(b)
     if da is None or db is None:
         return False
@@ -83,7 +92,7 @@ def _apart(a, b):
 
 def _check_strided(grads, outs):
     """The library's refusals of overlaps, for lists with tensors that it gets as copies."""
-    if any(_folded(o) for o in outs):
+    if any(not o.is_contiguous() and _folded(o) for o in outs):
         raise ValueError("an output whose elements share memory")
     items = [(o.data_ptr(), _end(o), i, True, o) for i, o in enumerate(outs) if o.numel()]
     if outs is not grads:
