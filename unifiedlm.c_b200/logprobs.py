@@ -297,8 +297,8 @@ def _shaped(out, shape, top_k):
 
 def lm_head_logprobs(h, weight, tokens, top_k=0, precision="bf16"):
     """TokenLogprobs of `tokens` (...) under the logits h @ weight.T: h (..., D) fp32 or bf16, weight
-    (V, D) fp32 or bf16. "bf16" contracts bf16 operands (rounding fp32 ones), "fp32" fp32 ones; the
-    statistics are fp32. Gradients of h and weight flow from logprobs and entropy, in the types of h
+    (V, D) fp32 or bf16. "bf16" contracts bf16 operands (rounding fp32 ones; the logits' gradient goes
+    into its products in two bf16 parts, 16 digits), "fp32" fp32 ones; the statistics are fp32. Gradients of h and weight flow from logprobs and entropy, in the types of h
     and weight; the alternatives are not differentiable."""
     if weight.dim() != 2 or h.dim() < 1 or h.shape[-1] != weight.shape[1]:
         raise ValueError(f"h {tuple(h.shape)} and weight {tuple(weight.shape)} do not match")
